@@ -475,6 +475,61 @@ RGK_API int rgk_argmax(const void* x, int64_t M, int64_t V, int dtype, int* out,
 RGK_API int rgk_geglu_bias(const void* up, const void* bias, int64_t M, int64_t X, int dtype,
                            void* out, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * A selective state space layer: its short causal convolution and its recurrence, and the draw of the next
+ * token.  These have no counterpart in the reference; they stand beside rgk_conv1d_*, rgk_linear_scan
+ * and rgk_argmax.  float32 or bfloat16 (one rounding, of each output), any width; tensors need no alignment
+ * beyond their elements' (aligned ones are faster).  Strides are in elements; the last dimensions are dense.
+ *
+ * rgk_causal_conv: x [B,T,E] (rows at b * x_batch + t * x_token), w [W,E], W = 2, 3 or 4, bias [E] or NULL,
+ *   state_in [B,W-1,E] or NULL (zeros)  ->  y [B,T,E] dense, state_out [B,W-1,E] or NULL:
+ *   X = state_in ++ x;  y_t = act(bias + sum_j w[j] X[t - (W-1) + j]), act silu or none (RGK_CONV_ACT_*);
+ *   rows in front of the last document start (segment_pos == 0; segment_pos may be NULL) at or before t do
+ *   not count.  state_out = the last W-1 rows of X, zero where a document start lies behind them; it may
+ *   be state_in.  T may be 0.
+ * rgk_selective_scan: with D_t = softplus(dt_t + dt_bias) (or without the softplus), for every channel e of
+ *   group g = e / (E / groups) and its N states (1 to 256):
+ *     h_t[n] = exp(D_t a[e,n]) h_{t-1}[n] + D_t x_t b_t[g,n]  (a document start drops h_{t-1}),
+ *     y_t = (sum_n h_t[n] c_t[g,n] + d[e] x_t) silu(z_t).
+ *   x, dt, z (or NULL) [B,T,E], b, c [B,T,groups,N]; a [E,N], d [E] or NULL, dt_bias [E] or NULL and the
+ *   states [B,E,N] are float32.  state_in NULL: zeros; state_out: NULL, or it may be state_in.  T may be 0.
+ * rgk_sample: out [M] int32, one token for each row of logits [M,V] (rows row_stride apart; V up to 2^20).
+ *   Tokens are ordered by logit, the largest first, equal ones by index.  Kept are the first top_k of them (all for
+ *   top_k <= 0), of those, with weights exp((logit - largest) / temperature) rounded to multiples of 2^-44
+ *   (2^-42 from 2^18 tokens on), the shortest prefix with at least top_p of their weight (one at least;
+ *   all for top_p >= 1), of those the ones with at least min_p of the largest weight.  The token is the first, by index, up to which the kept weights sum
+ *   to more than uniforms[m] (in [0, 1)) times all of them.  A temperature of 0 (or less) takes the
+ *   first maximum.  NaN counts as -inf; neither is drawn; a row of nothing else gives 0.
+ *   Every setting is an array of M on the device, or NULL: the value beside it for all rows.
+ * ---------------------------------------------------------------------------------------------- */
+enum { RGK_CONV_ACT_NONE = 0, RGK_CONV_ACT_SILU = 1 };
+RGK_API int rgk_causal_conv(const void* x, int64_t x_batch, int64_t x_token, const void* segment_pos,
+                            int pos_dtype, const void* w, const void* bias, const void* state_in, int64_t B,
+                            int64_t T, int64_t E, int W, int act, int dtype, void* y, void* state_out,
+                            void* stream);
+
+typedef struct rgk_scan_inputs {
+  const void *x, *dt, *z, *b, *c;
+  int64_t x_batch, x_token, dt_batch, dt_token, z_batch, z_token, b_batch, b_token, c_batch, c_token;
+  const float *a, *d, *dt_bias;
+  int softplus;
+} rgk_scan_inputs;
+RGK_API int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int pos_dtype,
+                               const float* state_in, int64_t B, int64_t T, int64_t E, int groups, int N,
+                               int dtype, void* y, float* state_out, void* stream);
+
+typedef struct rgk_sample_settings {
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_value;
+  int top_k_value;
+  float top_p_value, min_p_value;
+} rgk_sample_settings;
+RGK_API int rgk_sample(const void* logits, int64_t M, int64_t V, int64_t row_stride, int dtype,
+                       const float* uniforms, const rgk_sample_settings* settings, int* out, void* stream);
+
 /* Scratch needed by the calls above for a problem of this size (an upper bound over the entry
  * points, so one buffer serves all of them).  Returns 0 on invalid arguments. */
 RGK_API size_t rgk_workspace_bytes(int64_t B, int64_t T, int64_t E, int dtype);

@@ -24,6 +24,7 @@ RGK_F32, RGK_BF16 = 0, 1
  RGK_ETIMEOUT, RGK_EBOUNDS) = 0, -1, -2, -3, -4, -5, -6, -7, -8
 RGK_I32, RGK_I64 = 0, 1
 ACT_NONE, ACT_GELU_TANH, ACT_GEGLU = 0, 1, 2
+CONV_ACT_NONE, CONV_ACT_SILU = 0, 1
 GATES_AUTO, GATES_SIMT, GATES_TCGEN05, GATES_FUSED, GATES_FUSED_EXACT = 0, 1, 2, 3, 4
 
 _vp, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
@@ -50,6 +51,20 @@ class RgkChannelParams(ctypes.Structure):
 class RgkAttentionParams(ctypes.Structure):
   """struct rgk_attention_params of include/rgk.h."""
   _fields_ = [(n, _vp) for n in ("q_w", "k_w", "v_w", "final_w", "final_b")]
+
+
+class RgkScanInputs(ctypes.Structure):
+  """struct rgk_scan_inputs of include/rgk.h."""
+  _fields_ = ([(n, _vp) for n in ("x", "dt", "z", "b", "c")] +
+              [(f"{n}_{of}", _i64) for n in ("x", "dt", "z", "b", "c") for of in ("batch", "token")] +
+              [(n, _vp) for n in ("a", "d", "dt_bias")] + [("softplus", _int)])
+
+
+class RgkSampleSettings(ctypes.Structure):
+  """struct rgk_sample_settings of include/rgk.h."""
+  _fields_ = ([(n, _vp) for n in ("temperature", "top_k", "top_p", "min_p")] +
+              [("temperature_value", ctypes.c_float), ("top_k_value", _int),
+               ("top_p_value", ctypes.c_float), ("min_p_value", ctypes.c_float)])
 
 
 # name -> (restype, argtypes); mirrors include/rgk.h declaration by declaration.
@@ -120,6 +135,11 @@ SIGNATURES = {
     "rgk_embed": (_int, [_vp, _int, _vp, _i64, _i64, _i64, ctypes.c_float, _int, _vp, _vp]),
     "rgk_logits": (_int, [_vp, _vp, _i64, _i64, _i64, ctypes.c_float, _int, _vp, _vp, _vp]),
     "rgk_argmax": (_int, [_vp, _i64, _i64, _int, _vp, _vp]),
+    "rgk_causal_conv": (_int, [_vp, _i64, _i64, _vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int,
+                               _vp, _vp, _vp]),
+    "rgk_selective_scan": (_int, [ctypes.POINTER(RgkScanInputs), _vp, _int, _vp, _i64, _i64, _i64, _int, _int,
+                                  _int, _vp, _vp, _vp]),
+    "rgk_sample": (_int, [_vp, _i64, _i64, _i64, _int, _vp, ctypes.POINTER(RgkSampleSettings), _vp, _vp]),
     "rgk_add_rmsnorm": (_int, [_vp, _vp, _vp, _i64, _i64, ctypes.c_float, _int, _vp, _vp, _vp]),
     "rgk_geglu_bias": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp]),
     "rgk_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),

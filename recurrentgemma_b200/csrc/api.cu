@@ -685,6 +685,108 @@ int rgk_argmax(const void* x, int64_t M, int64_t V, int dtype, int* out, void* s
   return RGK_OK;
 }
 
+// Common to the calls around a state space layer: sizes, and segment_pos where it is given.
+static int check_sequence(int64_t B, int64_t T, int64_t E, int dtype, const void* pos, int pos_dtype) {
+  RGK_REQUIRE(dtype == RGK_F32 || dtype == RGK_BF16, RGK_EINVAL, "unknown dtype %d", dtype);
+  RGK_REQUIRE(pos == nullptr || pos_dtype == RGK_I32 || pos_dtype == RGK_I64, RGK_EINVAL, "unknown pos dtype %d",
+              pos_dtype);
+  RGK_REQUIRE(B >= 0 && T >= 0 && E >= 0, RGK_EINVAL, "negative size (B=%lld T=%lld E=%lld)", (long long)B,
+              (long long)T, (long long)E);
+  RGK_REQUIRE(B <= 65535, RGK_ESHAPE, "batch %lld exceeds 65535", (long long)B);
+  RGK_REQUIRE(T < ((int64_t)1 << 31), RGK_ESHAPE, "sequence length %lld exceeds 2^31 - 1", (long long)T);
+  RGK_REQUIRE(E <= (1 << 20), RGK_ESHAPE, "width %lld exceeds 2^20", (long long)E);
+  return RGK_OK;
+}
+static bool aligned_to(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)size == 0; }
+
+int rgk_causal_conv(const void* x, int64_t x_batch, int64_t x_token, const void* segment_pos, int pos_dtype,
+                    const void* w, const void* bias, const void* state_in, int64_t B, int64_t T, int64_t E,
+                    int W, int act, int dtype, void* y, void* state_out, void* stream) {
+  const int rc = check_sequence(B, T, E, dtype, segment_pos, pos_dtype);
+  if (rc != RGK_OK) return rc;
+  RGK_REQUIRE(W >= 2 && W <= 4, RGK_ESHAPE, "%d taps: 2, 3 and 4 are covered", W);
+  RGK_REQUIRE(act == RGK_CONV_ACT_NONE || act == RGK_CONV_ACT_SILU, RGK_EINVAL, "unknown activation %d", act);
+  if (B == 0 || E == 0) return RGK_OK;
+  RGK_REQUIRE(w && (T == 0 || (x && y)), RGK_EINVAL, "NULL pointer argument");
+  const int size = elem_size(dtype);
+  RGK_REQUIRE(aligned_to(x, size) && aligned_to(w, size) && aligned_to(bias, size) && aligned_to(state_in, size) &&
+                  aligned_to(y, size) && aligned_to(state_out, size), RGK_EALIGN,
+              "a pointer is not aligned to its elements");
+  if (T == 0 && state_out == nullptr) return RGK_OK;
+  RGK_CHECK_DEVICE();
+  rgk::ConvArgs p = {};
+  p.x = x; p.x_batch = x_batch; p.x_token = x_token;
+  p.pos = segment_pos; p.pos64 = pos_dtype == RGK_I64;
+  p.w = w; p.bias = bias; p.state_in = state_in;
+  p.B = B; p.T = T; p.E = E;
+  p.taps = W; p.silu = act == RGK_CONV_ACT_SILU;
+  p.y = y; p.state_out = state_out;
+  RGK_CUDA(rgk::launch_causal_conv(p, dtype, static_cast<cudaStream_t>(stream)), "causal conv launch");
+  return RGK_OK;
+}
+
+int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int pos_dtype, const float* state_in,
+                       int64_t B, int64_t T, int64_t E, int groups, int N, int dtype, void* y, float* state_out,
+                       void* stream) {
+  const int rc = check_sequence(B, T, E, dtype, segment_pos, pos_dtype);
+  if (rc != RGK_OK) return rc;
+  RGK_REQUIRE(in != nullptr, RGK_EINVAL, "in is NULL");
+  RGK_REQUIRE(N >= 1 && N <= 256, RGK_ESHAPE, "%d states a channel: 1 to 256 are covered", N);
+  RGK_REQUIRE(groups >= 1 && E % groups == 0, RGK_ESHAPE, "width %lld is not divisible by %d groups", (long long)E,
+              groups);
+  if (B == 0 || E == 0) return RGK_OK;
+  RGK_REQUIRE(in->a && (T == 0 || (in->x && in->dt && in->b && in->c && y)), RGK_EINVAL, "NULL pointer argument");
+  const int size = elem_size(dtype);
+  RGK_REQUIRE(aligned_to(in->x, size) && aligned_to(in->dt, size) && aligned_to(in->z, size) && aligned_to(in->b, size) &&
+                  aligned_to(in->c, size) && aligned_to(y, size) && aligned_to(in->a, 4) && aligned_to(in->d, 4) &&
+                  aligned_to(in->dt_bias, 4) && aligned_to(state_in, 4) && aligned_to(state_out, 4), RGK_EALIGN,
+              "a pointer is not aligned to its elements");
+  if (T == 0 && state_out == nullptr) return RGK_OK;
+  RGK_CHECK_DEVICE();
+  rgk::SelectiveArgs p = {};
+  p.x = in->x; p.dt = in->dt; p.z = in->z; p.b = in->b; p.c = in->c;
+  p.x_batch = in->x_batch; p.x_token = in->x_token;
+  p.dt_batch = in->dt_batch; p.dt_token = in->dt_token;
+  p.z_batch = in->z_batch; p.z_token = in->z_token;
+  p.b_batch = in->b_batch; p.b_token = in->b_token;
+  p.c_batch = in->c_batch; p.c_token = in->c_token;
+  p.a = in->a; p.d = in->d; p.dt_bias = in->dt_bias; p.softplus = in->softplus;
+  p.pos = segment_pos; p.pos64 = pos_dtype == RGK_I64;
+  p.state_in = state_in;
+  p.B = B; p.T = T; p.E = E; p.groups = groups; p.N = N;
+  p.y = y; p.state_out = state_out;
+  RGK_CUDA(rgk::launch_selective_scan(p, dtype, static_cast<cudaStream_t>(stream)), "selective scan launch");
+  return RGK_OK;
+}
+
+int rgk_sample(const void* logits, int64_t M, int64_t V, int64_t row_stride, int dtype, const float* uniforms,
+               const rgk_sample_settings* settings, int* out, void* stream) {
+  RGK_REQUIRE(dtype == RGK_F32 || dtype == RGK_BF16, RGK_EINVAL, "unknown dtype %d", dtype);
+  RGK_REQUIRE(M >= 0 && M < ((int64_t)1 << 27) && V >= 1, RGK_EINVAL, "bad size (M=%lld V=%lld)", (long long)M,
+              (long long)V);
+  RGK_REQUIRE(V <= (1 << 20), RGK_ESHAPE, "%lld tokens: up to 2^20 are covered", (long long)V);
+  RGK_REQUIRE(settings != nullptr, RGK_EINVAL, "settings is NULL");
+  if (M == 0) return RGK_OK;
+  RGK_REQUIRE(logits && uniforms && out, RGK_EINVAL, "NULL pointer argument");
+  RGK_REQUIRE(aligned_to(logits, elem_size(dtype)) && aligned_to(uniforms, 4) && aligned_to(out, 4) &&
+                  aligned_to(settings->temperature, 4) && aligned_to(settings->top_k, 4) &&
+                  aligned_to(settings->top_p, 4) && aligned_to(settings->min_p, 4), RGK_EALIGN,
+              "a pointer is not aligned to its elements");
+  RGK_CHECK_DEVICE();
+  rgk::SampleArgs p = {};
+  p.logits = logits; p.M = M; p.V = V; p.row_stride = row_stride;
+  p.uniforms = uniforms;
+  p.temperature = settings->temperature; p.top_k = settings->top_k;
+  p.top_p = settings->top_p; p.min_p = settings->min_p;
+  p.temperature_value = settings->temperature_value; p.top_k_value = settings->top_k_value;
+  p.top_p_value = settings->top_p_value; p.min_p_value = settings->min_p_value;
+  p.bits = 44;                              // a row's weights sum to 2^62 at most
+  while (p.bits > 42 && (V << p.bits) > ((int64_t)1 << 62)) --p.bits;
+  p.out = out;
+  RGK_CUDA(rgk::launch_sample(p, dtype, static_cast<cudaStream_t>(stream)), "sample launch");
+  return RGK_OK;
+}
+
 int rgk_geglu_bias(const void* up, const void* bias, int64_t M, int64_t X, int dtype, void* out,
                    void* stream) {
   RGK_REQUIRE(dtype == RGK_F32 || dtype == RGK_BF16, RGK_EINVAL, "unknown dtype %d", dtype);

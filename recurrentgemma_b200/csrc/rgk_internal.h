@@ -321,4 +321,55 @@ cudaError_t launch_decode_update(const void* a, const void* xn, const float* h_i
                                  int64_t B, int64_t E, int dtype, void* out, float* h_out,
                                  cudaStream_t s);
 
+// causal_conv.cu (strides in elements)
+struct ConvArgs {
+  const void* x;
+  int64_t x_batch, x_token;
+  const void* pos;                       // or NULL: no document starts
+  int pos64;
+  const void* w;
+  const void* bias;                      // or NULL
+  const void* state_in;                  // or NULL: nothing in front
+  int64_t B, T, E;
+  int taps, silu;
+  void* y;
+  void* state_out;                       // or NULL
+  int64_t chunks;                        // of a sequence (set by the launcher)
+};
+cudaError_t launch_causal_conv(const ConvArgs& p, int dtype, cudaStream_t s);
+
+// selective_scan.cu (strides in elements)
+struct SelectiveArgs {
+  const void *x, *dt, *z, *b, *c;        // z: or NULL
+  int64_t x_batch, x_token, dt_batch, dt_token, z_batch, z_token, b_batch, b_token, c_batch, c_token;
+  const float *a, *d, *dt_bias;          // d, dt_bias: or NULL
+  int softplus;
+  const void* pos;                       // or NULL: no document starts
+  int pos64;
+  const float* state_in;                 // or NULL: zeros
+  int64_t B, T, E;
+  int groups, N;
+  void* y;
+  float* state_out;                      // or NULL
+  int per_group, copy_x, copy_n, store4; // set by the launcher
+};
+cudaError_t launch_selective_scan(SelectiveArgs p, int dtype, cudaStream_t s);
+
+// sample.cu: a setting is read from its array, one for each row, or where that is NULL is the value
+struct SampleArgs {
+  const void* logits;
+  int64_t M, V, row_stride;
+  const float* uniforms;
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_value;
+  int top_k_value;
+  float top_p_value, min_p_value;
+  int bits;                              // of a weight's fraction
+  int* out;
+};
+cudaError_t launch_sample(const SampleArgs& p, int dtype, cudaStream_t s);
+
 }  // namespace rgk
