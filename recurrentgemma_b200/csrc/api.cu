@@ -727,7 +727,7 @@ int rgk_causal_conv(const void* x, int64_t x_batch, int64_t x_token, const void*
 
 int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int pos_dtype, const float* state_in,
                        int64_t B, int64_t T, int64_t E, int groups, int N, int dtype, void* y, float* state_out,
-                       void* stream) {
+                       void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_sequence(B, T, E, dtype, segment_pos, pos_dtype);
   if (rc != RGK_OK) return rc;
   RGK_REQUIRE(in != nullptr, RGK_EINVAL, "in is NULL");
@@ -741,9 +741,13 @@ int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int p
                   aligned_to(in->c, size) && aligned_to(y, size) && aligned_to(in->a, 4) && aligned_to(in->d, 4) &&
                   aligned_to(in->dt_bias, 4) && aligned_to(state_in, 4) && aligned_to(state_out, 4), RGK_EALIGN,
               "a pointer is not aligned to its elements");
+  RGK_REQUIRE(workspace == nullptr || workspace_bytes >= rgk::selective_workspace_bytes(), RGK_EWORKSPACE,
+              "workspace of %zu bytes, %zu needed", workspace_bytes, rgk::selective_workspace_bytes());
+  RGK_REQUIRE(aligned_to(workspace, 256), RGK_EALIGN, "the workspace must be 256-byte aligned");
   if (T == 0 && state_out == nullptr) return RGK_OK;
   RGK_CHECK_DEVICE();
   rgk::SelectiveArgs p = {};
+  p.header = static_cast<rgk::WsHeader*>(workspace);
   p.x = in->x; p.dt = in->dt; p.z = in->z; p.b = in->b; p.c = in->c;
   p.x_batch = in->x_batch; p.x_token = in->x_token;
   p.dt_batch = in->dt_batch; p.dt_token = in->dt_token;
@@ -758,6 +762,8 @@ int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int p
   RGK_CUDA(rgk::launch_selective_scan(p, dtype, static_cast<cudaStream_t>(stream)), "selective scan launch");
   return RGK_OK;
 }
+
+size_t rgk_selective_scan_workspace_bytes(void) { return rgk::selective_workspace_bytes(); }
 
 int rgk_sample(const void* logits, int64_t M, int64_t V, int64_t row_stride, int dtype, const float* uniforms,
                const rgk_sample_settings* settings, int* out, void* stream) {

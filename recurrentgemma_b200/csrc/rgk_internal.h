@@ -338,6 +338,7 @@ struct ConvArgs {
 };
 cudaError_t launch_causal_conv(const ConvArgs& p, int dtype, cudaStream_t s);
 
+struct WsHeader;
 // selective_scan.cu (strides in elements)
 struct SelectiveArgs {
   const void *x, *dt, *z, *b, *c;        // z: or NULL
@@ -351,8 +352,13 @@ struct SelectiveArgs {
   int groups, N;
   void* y;
   float* state_out;                      // or NULL
-  int per_group, copy_x, copy_n, store4; // set by the launcher
+  WsHeader* header;               // or NULL: time is not cut into chunks
+  int per_group, copy_x, copy_n, store4; // set by the launcher, like what follows
+  int blocks_per_group;
+  int64_t blocks, chunk, chunks;         // of channels; of time: length and number
+  int* done;                             // chunks that a block has done
 };
+size_t selective_workspace_bytes();
 cudaError_t launch_selective_scan(SelectiveArgs p, int dtype, cudaStream_t s);
 
 // sample.cu: a setting is read from its array, one for each row, or where that is NULL is the value

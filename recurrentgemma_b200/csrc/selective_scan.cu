@@ -5,23 +5,32 @@
 //
 // Bound: the special functions.  An (element, state) takes one exponential and four multiply-adds' worth of
 // float32 work, and an SM has 16 special-function results a clock but 128 multiply-adds: for 16 states (and
-// two functions each for softplus and silu) 168 M elements take 0.75 ms where their bytes take 0.21.
+// three more for softplus and silu) 168 M elements take 0.71 ms where their bytes take 0.21.  8 x 4096 x 5120 in
+// bfloat16: 988 us, 72 % of that rate.
 //
 // The recurrence runs in time order in registers: L neighbouring lanes share a channel, each with S of its
-// states, and time is not split - the lanes are, which leaves no work to do twice.  A CTA walks over tiles of
-// 32 time steps: (1) the raw tile, brought in by cp.async while the one before is worked on, becomes D and
-// D x in float32 (the softplus once an element, shared by all threads), b and c are widened; (2) the recurrence,
-// which reads those as broadcasts and leaves sums over its S states, joined over the L lanes by exchanging
-// halves of four time steps (three shuffles for four steps and the first four lanes, not eight); (3) d x, the gate
-// and the store, again by element.
+// states, and time is not split - the lanes are, which leaves no work to do twice.  A CTA is two teams of 128 threads.
+// The owners of the states do nothing but the recurrence, from float32 tiles in shared memory, and leave sums over
+// their S states; the helpers turn the next tile (brought in by cp.async) into D, D x and widened b and c, and the sums of the tile
+// before into outputs, so that one team's latencies lie under the other's work (one team for all three, tile
+// after tile: 1023 us and, for one row of 2048 steps, 190 where the teams take 134).  A load from shared memory costs what
+// arrives in registers, broadcast or not: a thread with two channels uses b and c twice (988 us; with one 1039, with 4
+// states 1325).  Polynomials in place of a quarter of the exponentials made it slower (1104), and a shuffle's latency
+// more than the parts of the sums in shared memory.
+//
+// Long calls of more channels than the CTAs hold are cut into chunks of time that are drawn by a ticket, so that no SM
+// works on a fifth CTA while others have four (1090 -> 1023 us in the form with one team); a state goes from chunk to chunk through state_out.
+#include <type_traits>
+
 #include "rgk_common.cuh"
 #include "rgk_internal.h"
 
 namespace rgk {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kTile = 32;                                        // time steps; one bit each in a warp's vote
+constexpr int kTeam = 128;                                        // threads of each half of a CTA
+constexpr int kMostBlocks = 1 << 16;                             // whose progress the workspace has room for
+constexpr unsigned kWaitLimit = 1u << 23;                       // polls, 0.2 us and more each
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float v) {
@@ -30,27 +39,58 @@ __device__ __forceinline__ float exp2_fast(float v) {
   return r;
 }
 
-// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1]: log1p(e) / e by a polynomial fitted for the
-// smallest largest relative error on [0, 1] (5e-9; 1.8e-7 in float32 arithmetic).  Steps of 1e-3 come out with their relative
-// precision, which the hardware logarithm of 1 + e would lose.
-__device__ __forceinline__ float softplus_step(float v) {
-  const float e = exp2_fast(-fabsf(v) * kLog2e);
-  float p = -0.0032440212089568377f;
-  p = fmaf(p, e, 0.01985144428908825f);
-  p = fmaf(p, e, -0.056959498673677444f);
-  p = fmaf(p, e, 0.10603651404380798f);
-  p = fmaf(p, e, -0.15305590629577637f);
-  p = fmaf(p, e, 0.1967593878507614f);
-  p = fmaf(p, e, -0.24954134225845337f);
-  p = fmaf(p, e, 0.3332996368408203f);
-  p = fmaf(p, e, -0.4999990165233612f);
-  p = fmaf(p, e, 1.0f);
-  return fmaf(p, e, v > 0.0f ? v : 0.0f);                        // (a NaN stays one: e is)
+// Two float32 operations in one instruction, on pairs as they lie in memory: half the issue slots of the same work
+// (the multiply-add pipe itself takes as long for a pair as for two).
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 split(Pair v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
-__device__ __forceinline__ float silu_fast(float v) { return __fdividef(v, 1.0f + exp2_fast(-v * kLog2e)); }
+__device__ __forceinline__ Pair exp2_pair(Pair x) {
+  const float2 v = split(x);
+  return pair(exp2_fast(v.x), exp2_fast(v.y));
+}
 
-template <typename T> __device__ __forceinline__ float widen1(T v) { return static_cast<float>(v); }
+// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1]: log1p(e) / e by a polynomial fitted for the
+// smallest largest relative error on [0, 1] (5e-9; 1.8e-7 in float32 arithmetic).  Steps of 1e-3 come out with their
+// relative precision, which the hardware logarithm of 1 + e would lose.  (A NaN stays one: e is.)
+__device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
+  const float2 arg = split(mul2(pair(fabsf(v0), fabsf(v1)), pair(-kLog2e, -kLog2e)));
+  const Pair e = pair(exp2_fast(arg.x), exp2_fast(arg.y));
+  constexpr float k[10] = {1.0f, -0.4999990165233612f, 0.3332996368408203f, -0.24954134225845337f,
+                           0.1967593878507614f, -0.15305590629577637f, 0.10603651404380798f,
+                           -0.056959498673677444f, 0.01985144428908825f, -0.0032440212089568377f};
+  Pair p = pair(k[9], k[9]);
+#pragma unroll
+  for (int i = 8; i >= 0; --i) p = fma2(p, e, pair(k[i], k[i]));
+  return split(fma2(p, e, pair(fmaxf(v0, 0.0f), fmaxf(v1, 0.0f))));
+}
+
+__device__ __forceinline__ float2 silu_fast(float v0, float v1) {
+  const float2 arg = split(mul2(pair(v0, v1), pair(-kLog2e, -kLog2e)));
+  float r0, r1;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(1.0f + exp2_fast(arg.x)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(1.0f + exp2_fast(arg.y)));
+  return split(mul2(pair(v0, v1), pair(r0, r1)));
+}
+
 // four consecutive elements, at an address aligned to four of them
 __device__ __forceinline__ void widen4(const __nv_bfloat16* p, float* f) {
   const uint2 v = *reinterpret_cast<const uint2*>(p);
@@ -72,237 +112,496 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src, bool ther
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" :: "r"(d), "l"(src), "n"(kBytes), "r"(n) : "memory");
 }
 
-// kTile rows of `width` elements (a multiple of the copies' size) into rows of `pitch`; rows from `rows` on and
-// elements from `there` on become zero.  kBytes: of one copy; sizeof(T) < 4: plain loads.
-template <typename T, int kBytes>
-__device__ __forceinline__ void fetch(T* dst, int pitch, const T* src, int64_t stride, int rows, int width, int there) {
-  constexpr int kPer = kBytes / (int)sizeof(T);
-  const int per_row = width / kPer;
-  for (int i = threadIdx.x; i < kTile * per_row; i += kThreads) {
-    const int r = i / per_row, e = (i - r * per_row) * kPer;
+// kRows rows into rows of kPitch elements; rows from `rows` on and elements from `there` on become zero (elements
+// from `width` on stay as they are).  kBytes: of one copy; 2: plain loads.
+template <typename T, int kBytes, int kThreads, int kRows, int kPitch>
+__device__ __forceinline__ void fetch(int tid, T* dst, const T* src, int64_t stride, int rows, int width, int there) {
+  constexpr int kPer = kBytes / (int)sizeof(T), kCols = kPitch / kPer;
+  static_assert(kPitch % kPer == 0, "whole copies");
+#pragma unroll
+  for (int k = 0; k < (kRows * kCols + kThreads - 1) / kThreads; ++k) {
+    const int i = tid + k * kThreads;
+    const int r = i / kCols, e = i % kCols * kPer;
+    if ((kRows * kCols % kThreads != 0 && r >= kRows) || e >= width) continue;
     const bool in = r < rows && e < there;
     const T* s = in ? src + r * stride + e : src;
-    if constexpr (kBytes >= 4) copy_async<kBytes>(dst + r * pitch + e, s, in);
-    else dst[r * pitch + e] = in ? *s : T(0.0f);
+    if constexpr (kBytes >= 4) copy_async<kBytes>(dst + r * kPitch + e, s, in);
+    else dst[r * kPitch + e] = in ? *s : T(0.0f);
   }
 }
-template <typename T>
-__device__ __forceinline__ void fetch_rows(int bytes, T* dst, int pitch, const T* src, int64_t stride, int rows,
-                                           int width, int there) {
-  if (bytes == 16) fetch<T, 16>(dst, pitch, src, stride, rows, width, there);
-  else if (bytes == 8) fetch<T, 8>(dst, pitch, src, stride, rows, width, there);
-  else if (bytes == 4) fetch<T, 4>(dst, pitch, src, stride, rows, width, there);
-  else fetch<T, sizeof(T) == 4 ? 4 : 2>(dst, pitch, src, stride, rows, width, there);
+// `bytes`: the largest copy that all addresses allow; kAligned: it is 16, or a whole row
+template <typename T, bool kAligned, int kThreads, int kRows, int kPitch>
+__device__ __forceinline__ void fetch_rows(int tid, int bytes, T* dst, const T* src, int64_t stride, int rows, int width,
+                                           int there) {
+  constexpr int kMost = kPitch * (int)sizeof(T) < 16 ? kPitch * (int)sizeof(T) : 16;
+  if (kAligned || bytes >= kMost) fetch<T, kMost, kThreads, kRows, kPitch>(tid, dst, src, stride, rows, width, there);
+  else if (sizeof(T) == 4 || bytes >= 4) fetch<T, 4, kThreads, kRows, kPitch>(tid, dst, src, stride, rows, width, there);
+  else fetch<T, (int)sizeof(T), kThreads, kRows, kPitch>(tid, dst, src, stride, rows, width, there);
 }
 
-// Shared memory: two stages of raw x, dt, z, b, c; then D and D x, y, b and c in float32.
-template <typename T, int S, int L> struct Smem {
-  static constexpr int kChan = kThreads / L;                     // channels of a CTA
+// Named barriers of a CTA: `arrive` does not wait, `meet` does.
+enum { kFull = 1, kDone = 3, kHelpersMeet = 5, kOwnersMeet = 6 };           // kFull, kDone: one for each of two buffers
+template <int kCount> __device__ __forceinline__ void arrive(int id) {
+  asm volatile("bar.arrive %0, %1;" :: "r"(id), "n"(kCount) : "memory");
+}
+template <int kCount> __device__ __forceinline__ void meet(int id) {
+  asm volatile("bar.sync %0, %1;" :: "r"(id), "n"(kCount) : "memory");
+}
+
+// S states of each of C channels a thread, L lanes a channel, kTile time steps a tile.  128 threads run the recurrence
+// (the owners of the states), 128 do what goes by element.  Shared memory: three stages of raw x, dt, z, b, c; two
+// buffers each of D and D x, parts of sums, b and c in float32.  In what is by channel and float32, channel
+// 4 q + k lies at k * kQuads + q: threads that work on four neighbouring channels store each of them next to what
+// their neighbours store.
+template <typename T, int S_, int C_, int L_, int kTile_> struct Shape {
+  static constexpr int S = S_, C = C_, L = L_, kTile = kTile_;
+  static constexpr int kOwners = kTeam / L;                      // (groups of lanes)
+  static constexpr int kChan = kOwners * C, kQuads = kChan / 4;  // channels of a CTA
   static constexpr int kPad = S * L;                             // states, rounded up
-  static constexpr int kPitchY = kChan + 8;                      // the four rows that a warp writes at once on banks of their own
   static constexpr int kRow = kTile * kChan * (int)sizeof(T);
   static constexpr int kRowN = kTile * kPad * (int)sizeof(T);
   static constexpr int kStage = 3 * kRow + 2 * kRowN;
-  static constexpr int kOffStep = 2 * kStage;
-  static constexpr int kOffY = kOffStep + kTile * kChan * 8;
-  static constexpr int kOffB = kOffY + kTile * kPitchY * 4;
-  static constexpr int kOffC = kOffB + kTile * kPad * 4;
-  static constexpr int kBytes = kOffC + kTile * kPad * 4;
+  static constexpr int kStep = kTile * kChan * 8, kPart = kTile * kTeam * C * 4, kWide = kTile * kPad * 4;
+  static constexpr int kOffStep = 3 * kStage;
+  static constexpr int kOffPart = kOffStep + 2 * kStep;
+  static constexpr int kOffB = kOffPart + 2 * kPart;
+  static constexpr int kOffC = kOffB + 2 * kWide;
+  static constexpr int kBytes = kOffC + 2 * kWide;
+  static constexpr int kUnroll = 8;
+  static_assert(kChan % 4 == 0 && kTile <= 32 && kTile % kUnroll == 0 && kBytes <= 227 * 1024, "a tile");
 };
 
-template <typename T, int S, int L>
-__global__ void __launch_bounds__(kThreads)
-selective_scan_kernel(const SelectiveArgs p) {
-  using Sm = Smem<T, S, L>;
-  constexpr int kChan = Sm::kChan, kPad = Sm::kPad;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int64_t b = blockIdx.y;
-  const int blocks = (p.per_group + kChan - 1) / kChan;          // of a group
-  const int g = blockIdx.x / blocks, e0 = (blockIdx.x - g * blocks) * kChan;
-  const int there = min(kChan, p.per_group - e0);                // channels that exist
-  const int64_t first = (int64_t)g * p.per_group + e0;           // the CTA's first channel
+// Waits until chunk - 1 of a block of channels has left its states.  The CTA that has drawn it is running (items are
+// drawn in this order by CTAs that have started), and none waits for a later one.
+__device__ __forceinline__ void wait_for(const int* done, int chunk, WsHeader* header) {
+  if (threadIdx.x == 0) {
+    int seen = 0;
+    for (unsigned n = 0; n < kWaitLimit; ++n) {
+      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(done) : "memory");
+      if (seen >= chunk) break;
+      __nanosleep(200);
+    }
+    if (seen < chunk) atomicExch(&header->status, kStatusTimeout);
+  }
+  meet<kTeam>(kOwnersMeet);
+}
 
-  const T* x = static_cast<const T*>(p.x) + b * p.x_batch + first;
-  const T* dt = static_cast<const T*>(p.dt) + b * p.dt_batch + first;
-  const T* z = p.z == nullptr ? nullptr : static_cast<const T*>(p.z) + b * p.z_batch + first;
-  const T* bb = static_cast<const T*>(p.b) + b * p.b_batch + (int64_t)g * p.N;
-  const T* cc = static_cast<const T*>(p.c) + b * p.c_batch + (int64_t)g * p.N;
-  auto raw = [&](int stage, int which) { return reinterpret_cast<T*>(smem + stage * Sm::kStage + which * Sm::kRow); };
+template <typename T, typename Sh, bool kAligned>
+__global__ void __launch_bounds__(2 * kTeam, 2)
+selective_scan_kernel(const SelectiveArgs p) {
+  constexpr int S = Sh::S, C = Sh::C, L = Sh::L, kTile = Sh::kTile;
+  constexpr int kChan = Sh::kChan, kQuads = Sh::kQuads, kPad = Sh::kPad;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_item;
+  __shared__ uint32_t s_starts[2];
+  const bool helper = threadIdx.x >= kTeam;
+  const int tid = threadIdx.x % kTeam, lane = tid & 31;          // in its team
+  auto raw = [&](int stage, int which) { return reinterpret_cast<T*>(smem + stage * Sh::kStage + which * Sh::kRow); };
   auto raw_n = [&](int stage, int which) {
-    return reinterpret_cast<T*>(smem + stage * Sm::kStage + 3 * Sm::kRow + which * Sm::kRowN);
+    return reinterpret_cast<T*>(smem + stage * Sh::kStage + 3 * Sh::kRow + which * Sh::kRowN);
   };
-  float2* s_step = reinterpret_cast<float2*>(smem + Sm::kOffStep);
-  float* s_y = reinterpret_cast<float*>(smem + Sm::kOffY);
-  float* s_b = reinterpret_cast<float*>(smem + Sm::kOffB);
-  float* s_c = reinterpret_cast<float*>(smem + Sm::kOffC);
+  auto steps = [&](int buf) { return reinterpret_cast<float2*>(smem + Sh::kOffStep + buf * Sh::kStep); };
+  auto parts = [&](int buf) { return reinterpret_cast<float*>(smem + Sh::kOffPart + buf * Sh::kPart); };
+  auto wide_b = [&](int buf) { return reinterpret_cast<float*>(smem + Sh::kOffB + buf * Sh::kWide); };
+  auto wide_c = [&](int buf) { return reinterpret_cast<float*>(smem + Sh::kOffC + buf * Sh::kWide); };
 
   // the places of states that do not exist are never copied to: zero once
   if (p.N < kPad) {
-    for (int i = tid; i < 2 * kTile * kPad; i += kThreads) {
-      raw_n(0, 0)[i] = T(0.0f);
-      raw_n(1, 0)[i] = T(0.0f);
+    for (int stage = 0; stage < 3; ++stage) {
+      for (int i = threadIdx.x; i < 2 * kTile * kPad; i += 2 * kTeam) raw_n(stage, 0)[i] = T(0.0f);
     }
     __syncthreads();
   }
-  auto ask = [&](int64_t t0, int stage) {
-    const int rows = (int)min((int64_t)kTile, p.T - t0);
-    fetch_rows<T>(p.copy_x, raw(stage, 0), kChan, x + t0 * p.x_token, p.x_token, rows, kChan, there);
-    fetch_rows<T>(p.copy_x, raw(stage, 1), kChan, dt + t0 * p.dt_token, p.dt_token, rows, kChan, there);
-    if (z != nullptr) fetch_rows<T>(p.copy_x, raw(stage, 2), kChan, z + t0 * p.z_token, p.z_token, rows, kChan, there);
-    fetch_rows<T>(p.copy_n, raw_n(stage, 0), kPad, bb + t0 * p.b_token, p.b_token, rows, p.N, p.N);
-    fetch_rows<T>(p.copy_n, raw_n(stage, 1), kPad, cc + t0 * p.c_token, p.c_token, rows, p.N, p.N);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
 
-  // a thread's states: n = q * 4 L + l * 4 + i for its values 4 q + i (S = 4 Q; S < 4: n = l * S + i)
-  const int l = tid & (L - 1), ch = tid / L;
-  constexpr int kVec = S < 4 ? S : 4;
-  auto state_of = [&](int s) { return (s / kVec) * kVec * L + l * kVec + s % kVec; };
-  float h[S], a2[S];
+  const int64_t items = p.chunks * p.blocks;
+  for (int64_t item = blockIdx.x; item < items;) {
+    const int64_t chunk = item / p.blocks;
+    const int block = (int)(item - chunk * p.blocks);
+    const int per_row = p.groups * p.blocks_per_group;
+    const int64_t b = block / per_row;
+    const int in_row = block % per_row, g = in_row / p.blocks_per_group, e0 = (in_row - g * p.blocks_per_group) * kChan;
+    const int there = min(kChan, p.per_group - e0);              // channels that exist
+    const int64_t first = (int64_t)g * p.per_group + e0;         // the CTA's first channel
+    const int64_t begin = chunk * p.chunk, end = min(p.T, begin + p.chunk);
+    const int tiles = (int)((end - begin + kTile - 1) / kTile);
+
+    if (helper) {
+      constexpr int kRowsAtOnce = kTeam / kQuads;
+      constexpr int kPasses = kTile > kRowsAtOnce ? kTile / kRowsAtOnce : 1;
+      constexpr int kPassesN = (kTile * kPad + kTeam * 4 - 1) / (kTeam * 4);
+      const T* x = static_cast<const T*>(p.x) + b * p.x_batch + first;
+      const T* dt = static_cast<const T*>(p.dt) + b * p.dt_batch + first;
+      const T* z = p.z == nullptr ? nullptr : static_cast<const T*>(p.z) + b * p.z_batch + first;
+      const T* bb = static_cast<const T*>(p.b) + b * p.b_batch + (int64_t)g * p.N;
+      const T* cc = static_cast<const T*>(p.c) + b * p.c_batch + (int64_t)g * p.N;
+      T* y = static_cast<T*>(p.y) + b * p.T * p.E + first;
+      // whole tiles of whole rows: a thread's copies start at fixed places, a tile further each time
+      constexpr int kPer = 16 / (int)sizeof(T);
+      constexpr int kCols = kChan >= kPer ? kChan / kPer : 1, kColsN = kPad >= kPer ? kPad / kPer : 1;  // copies of a row
+      constexpr bool kQuick = kAligned && kChan >= kPer && kPad >= kPer && kTeam % kCols == 0 && kTeam % kColsN == 0;
+      constexpr int kStepX = kTeam / kCols, kStepN = kTeam / kColsN;                                     // rows at once
+      const int xr = tid / kCols, xc = tid % kCols * kPer, nr = tid / kColsN, nc = tid % kColsN * kPer;
+      const T *qx = x + (begin + xr) * p.x_token + xc, *qd = dt + (begin + xr) * p.dt_token + xc;
+      const T* qz = z == nullptr ? nullptr : z + (begin + xr) * p.z_token + xc;
+      const T *qb = bb + (begin + nr) * p.b_token + nc, *qc = cc + (begin + nr) * p.c_token + nc;
+      auto ask = [&](int tile) {
+        const int64_t t0 = begin + (int64_t)tile * kTile;
+        const int stage = tile % 3, rows = (int)min((int64_t)kTile, end - t0);
+        if (kQuick && rows == kTile && there == kChan) {
+          auto copy = [&](T* dst, const T* src, int64_t stride, auto at_once, int r) {
+            constexpr int kAtOnce = decltype(at_once)::value;
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const int n = state_of(s);
-    const bool in = ch < there && n < p.N;
-    a2[s] = in ? p.a[(first + ch) * p.N + n] * kLog2e : 0.0f;
-    h[s] = in && p.state_in != nullptr ? p.state_in[(b * p.E + first + ch) * p.N + n] : 0.0f;
-  }
+            for (int k = 0; k < (kTile + kAtOnce - 1) / kAtOnce; ++k) {
+              if (kTile % kAtOnce == 0 || r + k * kAtOnce < kTile) copy_async<16>(dst + k * kTeam * kPer, src + k * kAtOnce * stride, true);
+            }
+          };
+          std::integral_constant<int, kStepX> by_x;
+          std::integral_constant<int, kStepN> by_n;
+          copy(raw(stage, 0) + tid * kPer, qx, p.x_token, by_x, xr);
+          copy(raw(stage, 1) + tid * kPer, qd, p.dt_token, by_x, xr);
+          if (z != nullptr) copy(raw(stage, 2) + tid * kPer, qz, p.z_token, by_x, xr);
+          if (nc < p.N) {
+            copy(raw_n(stage, 0) + tid * kPer, qb, p.b_token, by_n, nr);
+            copy(raw_n(stage, 1) + tid * kPer, qc, p.c_token, by_n, nr);
+          }
+          qx += kTile * p.x_token; qd += kTile * p.dt_token; qb += kTile * p.b_token; qc += kTile * p.c_token;
+          if (z != nullptr) qz += kTile * p.z_token;
+        } else {
+          fetch_rows<T, kAligned, kTeam, kTile, kChan>(tid, p.copy_x, raw(stage, 0), x + t0 * p.x_token, p.x_token, rows, kChan, there);
+          fetch_rows<T, kAligned, kTeam, kTile, kChan>(tid, p.copy_x, raw(stage, 1), dt + t0 * p.dt_token, p.dt_token, rows, kChan, there);
+          if (z != nullptr)
+            fetch_rows<T, kAligned, kTeam, kTile, kChan>(tid, p.copy_x, raw(stage, 2), z + t0 * p.z_token, p.z_token, rows, kChan, there);
+          fetch_rows<T, kAligned, kTeam, kTile, kPad>(tid, p.copy_n, raw_n(stage, 0), bb + t0 * p.b_token, p.b_token, rows, p.N, p.N);
+          fetch_rows<T, kAligned, kTeam, kTile, kPad>(tid, p.copy_n, raw_n(stage, 1), cc + t0 * p.c_token, p.c_token, rows, p.N, p.N);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      auto starts_at = [&](int tile) {
+        const int64_t t = begin + (int64_t)tile * kTile + lane;
+        return p.pos != nullptr && lane < kTile && t < end && pos_is_zero(p.pos, p.pos64, b * p.T + t);
+      };
 
-  const int tiles = (int)((p.T + kTile - 1) / kTile);
-  if (tiles > 0) ask(0, 0);
-  for (int tile = 0; tile < tiles; ++tile) {
-    const int64_t t0 = (int64_t)tile * kTile;
-    const int stage = tile & 1, rows = (int)min((int64_t)kTile, p.T - t0);
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();                                             // the tile is here; the one before is done with
-    if (tile + 1 < tiles) ask(t0 + kTile, stage ^ 1);
-    uint32_t starts = 0;
-    if (p.pos != nullptr)
-      starts = __ballot_sync(0xffffffffu, lane < rows && pos_is_zero(p.pos, p.pos64, b * p.T + t0 + lane));
-
-    for (int i = tid; i < kTile * kChan / 4; i += kThreads) {
-      const int t = i / (kChan / 4), e = (i - t * (kChan / 4)) * 4;
-      float vx[4], vd[4], st[4];
-      widen4(raw(stage, 0) + t * kChan + e, vx);
-      widen4(raw(stage, 1) + t * kChan + e, vd);
+      const int q = tid % kQuads, row0 = tid / kQuads;           // a thread's four channels, 4 q to 4 q + 3
+      float bias[4], d[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float v = vd[k] + (p.dt_bias != nullptr && e + k < there ? p.dt_bias[first + e + k] : 0.0f);
-        // a step of no time leaves the states of a row that does not exist as they are
-        st[k] = t < rows ? (p.softplus ? softplus_step(v) : v) : 0.0f;
+        const bool in = 4 * q + k < there;
+        bias[k] = in && p.dt_bias != nullptr ? p.dt_bias[first + 4 * q + k] : 0.0f;
+        d[k] = in && p.d != nullptr ? p.d[first + 4 * q + k] : 0.0f;
       }
+      // what the recurrence reads of a tile
+      auto prepare = [&](int tile, bool start) {
+        const int stage = tile % 3, buf = tile & 1, rows = (int)min((int64_t)kTile, end - begin - (int64_t)tile * kTile);
+        if (tid < 32) {
+          const uint32_t all = __ballot_sync(0xffffffffu, start);
+          if (lane == 0) s_starts[buf] = all;
+        }
+        // (all that is read before anything that is written: to the compiler they may overlap)
+        float by_x[kPasses][4], by_step[kPasses][4], by_n[kPassesN][2][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s_step[t * kChan + e + k] = make_float2(st[k], t < rows ? st[k] * vx[k] : 0.0f);
-    }
-    for (int i = tid; i < kTile * kPad / kVec; i += kThreads) {
+        for (int k = 0; k < kPasses; ++k) {
+          const int t = row0 + k * kRowsAtOnce;
+          if (kRowsAtOnce > kTile && t >= kTile) break;
+          widen4(raw(stage, 0) + t * kChan + 4 * q, by_x[k]);
+          widen4(raw(stage, 1) + t * kChan + 4 * q, by_step[k]);
+        }
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        s_b[i * kVec + k] = widen1(raw_n(stage, 0)[i * kVec + k]);
-        s_c[i * kVec + k] = widen1(raw_n(stage, 1)[i * kVec + k]);
-      }
-    }
-    __syncthreads();
+        for (int k = 0; k < kPassesN; ++k) {
+          const int i = (tid + k * kTeam) * 4;
+          if (kTile * kPad % (kTeam * 4) != 0 && i >= kTile * kPad) break;
+          widen4(raw_n(stage, 0) + i, by_n[k][0]);
+          widen4(raw_n(stage, 1) + i, by_n[k][1]);
+        }
+#pragma unroll
+        for (int k = 0; k < kPassesN; ++k) {
+          const int i = (tid + k * kTeam) * 4;
+          if (kTile * kPad % (kTeam * 4) != 0 && i >= kTile * kPad) break;
+          *reinterpret_cast<float4*>(wide_b(buf) + i) = make_float4(by_n[k][0][0], by_n[k][0][1], by_n[k][0][2], by_n[k][0][3]);
+          *reinterpret_cast<float4*>(wide_c(buf) + i) = make_float4(by_n[k][1][0], by_n[k][1][1], by_n[k][1][2], by_n[k][1][3]);
+        }
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          const int t = row0 + k * kRowsAtOnce;
+          if (kRowsAtOnce > kTile && t >= kTile) break;
+          float (&vx)[4] = by_x[k], (&step)[4] = by_step[k];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) step[i] += bias[i];
+          if (p.softplus) {
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const float2 two = softplus_steps(step[i], step[i + 1]);
+              step[i] = two.x; step[i + 1] = two.y;
+            }
+          }
+          if (rows < kTile && t >= rows) {                       // a step of no time leaves the states as they are
+#pragma unroll
+            for (int i = 0; i < 4; ++i) step[i] = vx[i] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) steps(buf)[t * kChan + i * kQuads + q] = make_float2(step[i], step[i] * vx[i]);
+        }
+      };
+      // its outputs
+      auto finish = [&](int tile) {
+        const int64_t t0 = begin + (int64_t)tile * kTile;
+        const int stage = tile % 3, rows = (int)min((int64_t)kTile, end - t0);
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          const int t = row0 + k * kRowsAtOnce;
+          if (t >= rows || 4 * q >= there) continue;
+          float vx[4], out[4];
+          widen4(raw(stage, 0) + t * kChan + 4 * q, vx);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* part = parts(tile & 1) + (t * kChan + i * kQuads + q) * L;
+            float sum;
+            if constexpr (L == 1) {
+              sum = part[0];
+            } else if constexpr (L == 2) {
+              const float2 v = *reinterpret_cast<const float2*>(part);
+              sum = v.x + v.y;
+            } else {
+              sum = 0.0f;
+#pragma unroll
+              for (int j = 0; j < L; j += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(part + j);
+                sum += (v.x + v.y) + (v.z + v.w);
+              }
+            }
+            out[i] = fmaf(d[i], vx[i], sum);
+          }
+          if (z != nullptr) {
+            float vz[4];
+            widen4(raw(stage, 2) + t * kChan + 4 * q, vz);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const float2 gate = silu_fast(vz[i], vz[i + 1]);
+              out[i] *= gate.x; out[i + 1] *= gate.y;
+            }
+          }
+          T* to = y + (t0 + t) * p.E + 4 * q;
+          if (kAligned || (p.store4 && 4 * q + 4 <= there)) {
+            if constexpr (sizeof(T) == 2)
+              *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3]));
+            else
+              *reinterpret_cast<float4*>(to) = make_float4(out[0], out[1], out[2], out[3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (4 * q + i < there) to[i] = static_cast<T>(out[i]);
+            }
+          }
+        }
+      };
 
+      // While the owners work on tile - 1: tile's inputs, then the outputs of tile - 1.  A buffer is written again two
+      // tiles later, when the owners have long met for the tile in between.
+      if (tiles > 0) ask(0);
+      bool start = starts_at(0);
 #pragma unroll 1
-    for (int t = 0; t < kTile; t += 4) {
-      float y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 step = s_step[(t + j) * kChan + ch];
-        if ((starts >> (t + j)) & 1u) {
-#pragma unroll
-          for (int s = 0; s < S; ++s) h[s] = 0.0f;
-        }
-        y[j] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const int n = state_of(s);
-          h[s] = fmaf(exp2_fast(step.x * a2[s]), h[s], step.y * s_b[(t + j) * kPad + n]);
-          y[j] = fmaf(h[s], s_c[(t + j) * kPad + n], y[j]);
+      for (int tile = 0; tile < tiles; ++tile) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        meet<kTeam>(kHelpersMeet);                               // the tile is here, tile - 2 is done with
+        if (tile + 1 < tiles) ask(tile + 1);
+        prepare(tile, start);
+        start = starts_at(tile + 1);
+        arrive<2 * kTeam>(kFull + (tile & 1));
+        if (tile > 0) {
+          meet<2 * kTeam>(kDone + ((tile - 1) & 1));
+          finish(tile - 1);
         }
       }
-      // sums over the channel's lanes: with every exchange a lane keeps half of its time steps
-      int mine = 0;
-      if constexpr (L >= 2) {
-        const bool up = l & 1;
-        const float g0 = __shfl_xor_sync(0xffffffffu, up ? y[0] : y[2], 1);
-        const float g1 = __shfl_xor_sync(0xffffffffu, up ? y[1] : y[3], 1);
-        y[0] = (up ? y[2] : y[0]) + g0;
-        y[1] = (up ? y[3] : y[1]) + g1;
-        mine = up ? 2 : 0;
+      if (tiles > 0) {
+        meet<2 * kTeam>(kDone + ((tiles - 1) & 1));
+        finish(tiles - 1);
       }
-      if constexpr (L >= 4) {
-        const bool up = l & 2;
-        const float g0 = __shfl_xor_sync(0xffffffffu, up ? y[0] : y[1], 2);
-        y[0] = (up ? y[1] : y[0]) + g0;
-        mine += up ? 1 : 0;
-      }
+    } else {
+      // A thread's channels, for each of its c the one at place owner + c * kOwners, and their states in runs of kRun
+      // that lie next to its neighbours' (value kRun r + i is state kRun L r + kRun l + i).
+      constexpr int kRun = S < 4 ? S : 4, kUnroll = Sh::kUnroll;
+      const int l = tid & (L - 1), owner = tid / L;
+      auto channel_of = [&](int c) { const int at = owner + c * Sh::kOwners; return at % kQuads * 4 + at / kQuads; };
+      auto state_of = [&](int s) { return s / kRun * kRun * L + l * kRun + s % kRun; };
+      if (chunk > 0) wait_for(p.done + block, (int)chunk, p.header);
+      const float* from = chunk > 0 ? p.state_out : p.state_in;
+      Pair h[C][S / 2], a2[C][S / 2];
 #pragma unroll
-      for (int o = 4; o < L; o <<= 1) y[0] += __shfl_xor_sync(0xffffffffu, y[0], o);
-      constexpr int kKept = L >= 4 ? 1 : L == 2 ? 2 : 4;
-      if (l < 4) {
+      for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int j = 0; j < kKept; ++j) s_y[(t + mine + j) * Sm::kPitchY + ch] = y[j];
+        for (int s = 0; s < S / 2; ++s) {
+          float va[2], vh[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int n = state_of(2 * s + i), ch = channel_of(c);
+            const bool in = ch < there && n < p.N;
+            va[i] = in ? p.a[(first + ch) * p.N + n] * kLog2e : 0.0f;
+            vh[i] = in && from != nullptr ? __ldcg(from + (b * p.E + first + ch) * p.N + n) : 0.0f;
+          }
+          a2[c][s] = pair(va[0], va[1]);
+          h[c][s] = pair(vh[0], vh[1]);
+        }
       }
+#pragma unroll 1
+      for (int tile = 0; tile < tiles; ++tile) {
+        const int buf = tile & 1;
+        meet<2 * kTeam>(kFull + buf);
+        const float2* s_step = steps(buf);
+        const float *s_b = wide_b(buf), *s_c = wide_c(buf);
+        float* s_part = parts(buf);
+        const uint32_t starts = s_starts[buf];
+        // (every lane leaves its part of a sum over states: the helpers join them, nothing here waits for another lane)
+        auto recur = [&](auto with_starts) {
+#pragma unroll 1
+          for (int t0 = 0; t0 < kTile; t0 += kUnroll) {
+            float sum[kUnroll][C];                               // (stored behind the loads of all of these steps)
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j) {
+              const int t = t0 + j, n = t * kPad + l * kRun;
+              Pair vb[S / 2], vc[S / 2];
+              if constexpr (S == 2) {
+                vb[0] = *reinterpret_cast<const Pair*>(s_b + n);
+                vc[0] = *reinterpret_cast<const Pair*>(s_c + n);
+              } else {
+#pragma unroll
+                for (int r = 0; r < S / 4; ++r) {
+                  const ulonglong2 b4 = *reinterpret_cast<const ulonglong2*>(s_b + n + r * 4 * L);
+                  const ulonglong2 c4 = *reinterpret_cast<const ulonglong2*>(s_c + n + r * 4 * L);
+                  vb[2 * r] = b4.x; vb[2 * r + 1] = b4.y;
+                  vc[2 * r] = c4.x; vc[2 * r + 1] = c4.y;
+                }
+              }
+#pragma unroll
+              for (int c = 0; c < C; ++c) {
+                const float2 step = s_step[t * kChan + owner + c * Sh::kOwners];
+                const Pair step2 = pair(step.x, step.x), put2 = pair(step.y, step.y);
+                Pair both = 0;
+#pragma unroll
+                for (int s = 0; s < S / 2; ++s) {
+                  const Pair arg = mul2(step2, a2[c][s]);
+                  Pair before = h[c][s];
+                  if (decltype(with_starts)::value && ((starts >> t) & 1u)) before = 0;
+                  h[c][s] = fma2(exp2_pair(arg), before, mul2(put2, vb[s]));
+                  both = s == 0 ? mul2(h[c][s], vc[s]) : fma2(h[c][s], vc[s], both);
+                }
+                const float2 halves = split(both);
+                sum[j][c] = halves.x + halves.y;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j) {
+#pragma unroll
+              for (int c = 0; c < C; ++c) s_part[((t0 + j) * C + c) * kTeam + tid] = sum[j][c];
+            }
+          }
+        };
+        if (starts != 0) recur(std::true_type{});
+        else recur(std::false_type{});
+        arrive<2 * kTeam>(kDone + buf);
+      }
+      if (p.state_out != nullptr) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int ch = channel_of(c);
+          if (ch >= there) continue;
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            const int n = state_of(s);
+            const float2 v = split(h[c][s / 2]);
+            if (n < p.N) p.state_out[(b * p.E + first + ch) * p.N + n] = s % 2 == 0 ? v.x : v.y;
+          }
+        }
+      }
+    }
+    if (p.chunks == 1) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      if (chunk + 1 < p.chunks) {
+        __threadfence();
+        asm volatile("st.release.gpu.global.s32 [%0], %1;" :: "l"(p.done + block), "r"((int)chunk + 1) : "memory");
+      }
+      s_item = (int)(atomicAdd(&p.header->ticket, 1u) + gridDim.x);
     }
     __syncthreads();
-
-    for (int i = tid; i < kTile * kChan / 4; i += kThreads) {
-      const int t = i / (kChan / 4), e = (i - t * (kChan / 4)) * 4;
-      if (t >= rows || e >= there) continue;
-      float vx[4], vz[4], out[4];
-      widen4(raw(stage, 0) + t * kChan + e, vx);
-      if (z != nullptr) widen4(raw(stage, 2) + t * kChan + e, vz);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        out[k] = s_y[t * Sm::kPitchY + e + k];
-        if (p.d != nullptr && e + k < there) out[k] = fmaf(p.d[first + e + k], vx[k], out[k]);
-        if (z != nullptr) out[k] *= silu_fast(vz[k]);
-      }
-      T* y = static_cast<T*>(p.y) + (b * p.T + t0 + t) * p.E + first + e;
-      if (p.store4 && e + 4 <= there) {
-        if constexpr (sizeof(T) == 2)
-          *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3]));
-        else
-          *reinterpret_cast<float4*>(y) = make_float4(out[0], out[1], out[2], out[3]);
-      } else {
-        for (int k = 0; k < 4 && e + k < there; ++k) y[k] = static_cast<T>(out[k]);
-      }
-    }
-  }
-
-  if (p.state_out != nullptr && ch < there) {
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int n = state_of(s);
-      if (n < p.N) p.state_out[(b * p.E + first + ch) * p.N + n] = h[s];
-    }
+    item = s_item;
   }
 }
 
-template <typename T, int S, int L>
-cudaError_t launch(SelectiveArgs p, cudaStream_t s) {
-  using Sm = Smem<T, S, L>;
+template <typename T, typename Sh, bool kAligned>
+cudaError_t launch_kernel(SelectiveArgs p, cudaStream_t s) {
   static PerDeviceOnce once;
-  const cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(selective_scan_kernel<T, S, L>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sm::kBytes);
-  });
+  int sms = 0;
+  cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(selective_scan_kernel<T, Sh, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kBytes);
+  }, &sms);
   if (e != cudaSuccess) return e;
-  p.copy_x = min(p.copy_x, Sm::kChan * (int)sizeof(T));
-  const int blocks = (p.per_group + Sm::kChan - 1) / Sm::kChan;
-  selective_scan_kernel<T, S, L><<<dim3((unsigned)(blocks * p.groups), (unsigned)p.B), kThreads, Sm::kBytes, s>>>(p);
+  p.blocks_per_group = (p.per_group + Sh::kChan - 1) / Sh::kChan;
+  p.blocks = (int64_t)p.blocks_per_group * p.groups * p.B;
+  p.chunk = p.T;
+  p.chunks = 1;
+  if (p.blocks >= ((int64_t)1 << 31)) return cudaErrorInvalidValue;
+  int64_t grid = p.blocks;
+  // Chunks of time drawn by a ticket.
+  if (p.header != nullptr && p.state_out != nullptr && p.T >= 512) {
+    int per_sm = 0;
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, selective_scan_kernel<T, Sh, kAligned>, 2 * kTeam,
+                                                           Sh::kBytes)) != cudaSuccess) return e;
+    const int64_t most = min((int64_t)per_sm, p.blocks / sms);
+    if (most > 0 && most * sms < p.blocks && p.blocks <= kMostBlocks) {
+      grid = most * sms;
+      p.chunk = max((int64_t)128, (p.T / 24 + Sh::kTile - 1) / Sh::kTile * Sh::kTile);
+      p.chunks = (p.T + p.chunk - 1) / p.chunk;
+      p.done = reinterpret_cast<int*>(p.header + 1);
+      if ((e = cudaMemsetAsync(&p.header->ticket, 0, sizeof(WsHeader) - sizeof(int) + p.blocks * sizeof(int), s)) != cudaSuccess)
+        return e;
+    }
+  }
+  selective_scan_kernel<T, Sh, kAligned><<<(unsigned)grid, 2 * kTeam, Sh::kBytes, s>>>(p);
   return cudaGetLastError();
 }
+template <typename T, int S, int C, int L, int kTile>
+cudaError_t launch(const SelectiveArgs& p, cudaStream_t s) {
+  using Sh = Shape<T, S, C, L, kTile>;
+  // (with whole copies of x's rows there are whole quads of channels too)
+  const bool aligned = p.copy_x >= min(16, Sh::kChan * (int)sizeof(T)) && p.copy_n >= min(16, Sh::kPad * (int)sizeof(T)) &&
+                       p.store4;
+  return aligned ? launch_kernel<T, Sh, true>(p, s) : launch_kernel<T, Sh, false>(p, s);
+}
 
+// What a shape takes, relative: `alone` is its time where every CTA has an SM (us for 2048 steps of 16 states), the
+// factor what blocks behind the first round of SMs add; a second CTA on an SM costs half as much as the first.
+double estimate(double alone, int64_t blocks, int sms) {
+  const double rounds = (double)blocks / sms;
+  return alone * (rounds <= 1.0 ? 1.0 : rounds < 2.0 ? rounds + 0.45 : rounds);
+}
+
+// Up to 16 states there is a choice: few states a thread keep a step short where channels are few, many states and
+// two channels share what is read from shared memory where they are many.  Measured in bfloat16, 2048 steps of 1280 /
+// 4096 / 5120 / 10240 / 15360 / 20480 channels: 2 states 70 / 183 / 154 / 292 / 430 / 569 us, 4 states 89 / 89 / 146 /
+// 193 / 282 / 372, 8 states 134 / 134 / 134 / 202 / 295 / 293, 8 of two channels 243 / 242 / 242 / 240 / 240 / 348;
+// 4096 steps of 40960 channels: 2026 / 1325 / 1039 / 988.
 template <typename T>
 cudaError_t launch_states(const SelectiveArgs& p, cudaStream_t s) {
-  if (p.N <= 4) return launch<T, 4, 1>(p, s);
-  if (p.N <= 8) return launch<T, 4, 2>(p, s);
-  if (p.N <= 16) return launch<T, 4, 4>(p, s);
-  if (p.N <= 32) return launch<T, 4, 8>(p, s);
-  if (p.N <= 64) return launch<T, 4, 16>(p, s);
-  if (p.N <= 128) return launch<T, 4, 32>(p, s);
-  return launch<T, 8, 32>(p, s);
+  if (p.N <= 4) return launch<T, 4, 1, 1, 16>(p, s);
+  if (p.N <= 8) return launch<T, 4, 1, 2, 16>(p, s);
+  if (p.N <= 16) {
+    static PerDeviceOnce once;
+    int sms = 0;
+    const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
+    if (e != cudaSuccess) return e;
+    auto blocks = [&](int channels) { return (p.per_group + channels - 1) / channels * p.groups * p.B; };
+    const double by[4] = {estimate(70, blocks(16), sms), estimate(89, blocks(32), sms), estimate(134, blocks(64), sms),
+                          estimate(242, blocks(128), sms)};
+    int best = 0;
+    for (int i = 1; i < 4; ++i) best = by[i] < by[best] ? i : best;
+    return best == 0   ? launch<T, 2, 1, 8, 32>(p, s)
+           : best == 1 ? launch<T, 4, 1, 4, 32>(p, s)
+           : best == 2 ? launch<T, 8, 1, 2, 16>(p, s)
+                       : launch<T, 8, 2, 2, 16>(p, s);
+  }
+  if (p.N <= 32) return launch<T, 4, 1, 8, 32>(p, s);
+  if (p.N <= 64) return launch<T, 4, 1, 16, 16>(p, s);
+  if (p.N <= 128) return launch<T, 4, 1, 32, 16>(p, s);
+  return launch<T, 8, 1, 32, 8>(p, s);
 }
 
 // The largest copy (bytes) that every address base + i * batch + j * token + k * width (elements) allows.
@@ -313,6 +612,8 @@ int copy_bytes(const void* base, int64_t batch, int64_t token, int64_t width, in
 }
 
 }  // namespace
+
+size_t selective_workspace_bytes() { return sizeof(WsHeader) + kMostBlocks * sizeof(int); }
 
 cudaError_t launch_selective_scan(SelectiveArgs p, int dtype, cudaStream_t s) {
   if (p.B == 0 || p.E == 0) return cudaSuccess;

@@ -120,7 +120,8 @@ def selective_scan(
       raise TypeError(f"a, d and dt_bias are float32 whatever the activations, got {p.dtype}")
   _check_state(state, (bs, e, n), torch.float32)
   pos = None if segment_pos is None else _pos(segment_pos, bs, l)
-  new_state = _new_state(state, (bs, e, n), torch.float32, dev, return_state, inplace)
+  # (long calls hand states from chunk to chunk in it, whether it is returned or not)
+  new_state = _new_state(state, (bs, e, n), torch.float32, dev, True, inplace)
   held = [None if t is None else _rows(t, 1) for t in (x, dt, z)] + [_rows(t, 2) for t in (b, c)]
   params = [None if p is None else p.contiguous() for p in (a, d, dt_bias)]
   sc = None if state is None else state.contiguous()
@@ -130,7 +131,9 @@ def selective_scan(
       *(s for t in held for s in ((0, 0) if t is None else (t.stride(0), t.stride(1)))),
       *(_lib.ptr(t) for t in params), int(softplus))
   with torch.cuda.device(dev):
-    _lib.check(_lib.load().rgk_selective_scan(
+    lib = _lib.load()
+    ws = _lib.workspace(dev, lib.rgk_selective_scan_workspace_bytes())
+    _lib.check(lib.rgk_selective_scan(
         ctypes.byref(p), _lib.ptr(pos), 0 if pos is None else _lib.pos_code(pos), _lib.ptr(sc), bs, l, e,
-        groups, n, code, y.data_ptr(), _lib.ptr(new_state), _lib.stream_ptr(dev)))
+        groups, n, code, y.data_ptr(), new_state.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
   return y, (new_state if return_state else None)
