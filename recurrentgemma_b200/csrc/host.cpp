@@ -41,6 +41,10 @@ struct Lib {
   decltype(&rgk_attention_block_prefill) attention_block_prefill;
   decltype(&rgk_mlp_workspace_bytes) mlp_workspace_bytes;
   decltype(&rgk_residual_channel) residual_channel;
+  decltype(&rgk_causal_conv) causal_conv;
+  decltype(&rgk_selective_scan) selective_scan;
+  decltype(&rgk_selective_scan_workspace_bytes) selective_scan_workspace_bytes;
+  decltype(&rgk_sample) sample;
 } g_lib;
 bool g_ready = false;
 
@@ -78,17 +82,21 @@ PyObject* not_here() {
   Py_RETURN_NOTIMPLEMENTED;
 }
 
-// A dense CUDA tensor argument; null if it is anything else (a tensor that has its operations in Python or
+// A strided CUDA tensor argument; null if it is anything else (a tensor that has its operations in Python or
 // no memory of its own - fake, batched, functional - among that).
-const at::Tensor* dense(PyObject* o) {
+const at::Tensor* strided(PyObject* o) {
   if (o == nullptr || !THPVariable_Check(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
   if (impl->is_python_dispatch() || !impl->has_storage() ||
       impl->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Functionalize, c10::DispatchKey::ZeroTensor})))
     return nullptr;
-  if (!t.is_cuda() || t.layout() != at::kStrided || !t.is_contiguous()) return nullptr;
+  if (!t.is_cuda() || t.layout() != at::kStrided) return nullptr;
   return &t;
+}
+const at::Tensor* dense(PyObject* o) {
+  const at::Tensor* t = strided(o);
+  return t == nullptr || !t->is_contiguous() ? nullptr : t;
 }
 
 // module.__dict__[name], borrowed (the module keeps it alive for the call); null if absent.  Modules hold
@@ -738,6 +746,150 @@ PyObject* block_step(PyObject* const* args, Py_ssize_t n) {
               PyObject_IsTrue(args[5]) == 1, PyObject_IsTrue(args[6]) == 1);
 }
 
+// ---- the operators of a state space layer, and sampling ---------------------------------------------
+// An optional dense tensor of the given type and sizes on x's device: absent, there, or something else.
+bool optional(PyObject* o, at::ScalarType dtype, const at::Tensor& x, at::IntArrayRef sizes, const at::Tensor** t) {
+  *t = nullptr;
+  if (o == Py_None) return true;
+  *t = dense(o);
+  return *t != nullptr && (*t)->scalar_type() == dtype && (*t)->device() == x.device() && (*t)->sizes() == sizes;
+}
+bool positions(PyObject* o, const at::Tensor& x, const at::Tensor** pos, int* code) {
+  *pos = nullptr;
+  *code = 0;
+  if (o == Py_None) return true;
+  *pos = dense(o);
+  if (*pos == nullptr || (*pos)->device() != x.device() || (*pos)->sizes() != x.sizes().slice(0, 2)) return false;
+  *code = pos_code(**pos);
+  return *code >= 0;
+}
+// A tensor of x's type and device whose rows [.., .., E] are dense.
+bool rows(const at::Tensor* t, const at::Tensor& x) {
+  return t != nullptr && t->scalar_type() == x.scalar_type() && t->device() == x.device() && t->sizes() == x.sizes() &&
+         t->stride(2) == 1;
+}
+const void* ptr(const at::Tensor* t) { return t == nullptr ? nullptr : t->const_data_ptr(); }
+const float* fptr(const at::Tensor* t) { return static_cast<const float*>(ptr(t)); }
+
+// (y, state): `given` where it was overwritten, None where it is not wanted
+PyObject* with_state(at::Tensor y, at::Tensor state, PyObject* given, bool inplace, bool want) {
+  Ref ry(wrap(std::move(y))), rs(!want ? Py_NewRef(Py_None) : inplace ? Py_NewRef(given) : wrap(std::move(state)));
+  return ry.p == nullptr || rs.p == nullptr ? nullptr : PyTuple_Pack(2, ry.p, rs.p);
+}
+
+// causal_conv(x, w, b, segment_pos, state, activation, return_state, inplace)
+PyObject* causal_conv(PyObject* const* args, Py_ssize_t n) {
+  if (!g_ready || n != 8) return not_here();
+  const at::Tensor *x = strided(args[0]), *w = dense(args[1]), *b, *pos, *state;
+  if (x == nullptr || w == nullptr || x->dim() != 3 || w->dim() != 2 || x->stride(2) != 1) return not_here();
+  const int64_t B = x->size(0), T = x->size(1), E = x->size(2), taps = w->size(0);
+  const int dt = dtype_code(x->scalar_type());
+  const bool silu = args[5] != Py_None, want = PyObject_IsTrue(args[6]) == 1, inplace = PyObject_IsTrue(args[7]) == 1;
+  int pc = 0;
+  if (dt < 0 || B * T * E == 0 || taps < 2 || taps > 4 || w->size(1) != E || w->scalar_type() != x->scalar_type() ||
+      w->device() != x->device() || (silu && (!PyUnicode_Check(args[5]) || PyUnicode_CompareWithASCIIString(args[5], "silu") != 0)) ||
+      !optional(args[2], x->scalar_type(), *x, {E}, &b) || !positions(args[3], *x, &pos, &pc) ||
+      !optional(args[4], x->scalar_type(), *x, {B, taps - 1, E}, &state) || (inplace && state == nullptr))
+    return not_here();
+  Guard guard(x->device().index());
+  const cudaStream_t s = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  at::Tensor y = empty({B, T, E}, x->scalar_type(), x->device()), made;
+  if (inplace) made = *state;
+  else if (want) made = empty({B, taps - 1, E}, x->scalar_type(), x->device());
+  if (!succeeded(g_lib.causal_conv(x->const_data_ptr(), x->stride(0), x->stride(1), ptr(pos), pc, w->const_data_ptr(), ptr(b),
+                                   ptr(state), B, T, E, (int)taps, silu ? RGK_CONV_ACT_SILU : RGK_CONV_ACT_NONE, dt,
+                                   y.mutable_data_ptr(), made.defined() ? made.mutable_data_ptr() : nullptr, s)))
+    return nullptr;
+  return with_state(std::move(y), std::move(made), args[4], inplace, want);
+}
+
+// selective_scan(x, dt, a, b, c, d, z, dt_bias, segment_pos, state, softplus, return_state, inplace)
+PyObject* selective_scan(PyObject* const* args, Py_ssize_t n) {
+  if (!g_ready || n != 13) return not_here();
+  const at::Tensor *x = strided(args[0]), *dt = strided(args[1]), *a = dense(args[2]), *b = strided(args[3]),
+                   *c = strided(args[4]), *z = args[6] == Py_None ? nullptr : strided(args[6]), *d, *bias, *pos, *state;
+  if (x == nullptr || a == nullptr || b == nullptr || c == nullptr || x->dim() != 3 || a->dim() != 2 || b->dim() != 4)
+    return not_here();
+  const int64_t B = x->size(0), T = x->size(1), E = x->size(2), N = a->size(1), G = b->size(2);
+  const int code = dtype_code(x->scalar_type());
+  const bool want = PyObject_IsTrue(args[11]) == 1, inplace = PyObject_IsTrue(args[12]) == 1;
+  int pc = 0;
+  auto by_group = [&](const at::Tensor* t) {
+    return t->scalar_type() == x->scalar_type() && t->device() == x->device() && t->sizes() == at::IntArrayRef({B, T, G, N}) &&
+           t->stride(3) == 1 && (G == 1 || t->stride(2) == N);
+  };
+  if (code < 0 || B * T * E == 0 || G < 1 || N < 1 || N > 256 || E % G != 0 || !rows(x, *x) || !rows(dt, *x) ||
+      (args[6] != Py_None && !rows(z, *x)) || !by_group(b) || !by_group(c) || a->scalar_type() != at::kFloat ||
+      a->device() != x->device() || a->size(0) != E || !optional(args[5], at::kFloat, *x, {E}, &d) ||
+      !optional(args[7], at::kFloat, *x, {E}, &bias) || !positions(args[8], *x, &pos, &pc) ||
+      !optional(args[9], at::kFloat, *x, {B, E, N}, &state) || (inplace && state == nullptr))
+    return not_here();
+  Guard guard(x->device().index());
+  const cudaStream_t s = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  Workspace ws;
+  if (T > 1 && !workspace(*x, s, g_lib.selective_scan_workspace_bytes(), &ws)) return nullptr;
+  at::Tensor y = empty({B, T, E}, x->scalar_type(), x->device());
+  // (long calls hand states from chunk to chunk in it, whether it is returned or not)
+  at::Tensor made = inplace ? *state : empty({B, E, N}, at::kFloat, x->device());
+  rgk_scan_inputs in = {};
+  in.x = ptr(x); in.dt = ptr(dt); in.z = ptr(z); in.b = ptr(b); in.c = ptr(c);
+  in.x_batch = x->stride(0); in.x_token = x->stride(1);
+  in.dt_batch = dt->stride(0); in.dt_token = dt->stride(1);
+  if (z != nullptr) { in.z_batch = z->stride(0); in.z_token = z->stride(1); }
+  in.b_batch = b->stride(0); in.b_token = b->stride(1);
+  in.c_batch = c->stride(0); in.c_token = c->stride(1);
+  in.a = fptr(a); in.d = fptr(d); in.dt_bias = fptr(bias);
+  in.softplus = PyObject_IsTrue(args[10]) == 1;
+  if (!succeeded(g_lib.selective_scan(&in, ptr(pos), pc, fptr(state), B, T, E, (int)G, (int)N, code, y.mutable_data_ptr(),
+                                      static_cast<float*>(made.mutable_data_ptr()), ws.ptr, ws.bytes, s)))
+    return nullptr;
+  return with_state(std::move(y), std::move(made), args[9], inplace, want);
+}
+
+// sample(logits, uniforms, temperature, top_k, top_p, min_p, out)
+PyObject* sample(PyObject* const* args, Py_ssize_t n) {
+  if (!g_ready || n != 7) return not_here();
+  const at::Tensor *x = strided(args[0]), *u = dense(args[1]);
+  if (x == nullptr || u == nullptr || x->dim() != 2 || x->stride(1) != 1) return not_here();
+  const int64_t M = x->size(0), V = x->size(1);
+  const int code = dtype_code(x->scalar_type());
+  if (code < 0 || M == 0 || V == 0 || u->scalar_type() != at::kFloat || u->device() != x->device() ||
+      u->sizes() != at::IntArrayRef({M}))
+    return not_here();
+  rgk_sample_settings set = {};
+  auto setting = [&](PyObject* o, const float** row, float* value) {
+    if (PyFloat_Check(o) || PyLong_Check(o)) {
+      *value = (float)PyFloat_AsDouble(o);
+      return !PyErr_Occurred() && *value >= 0.0f;
+    }
+    const at::Tensor* t = nullptr;
+    if (o == Py_None || !optional(o, at::kFloat, *x, {M}, &t)) return false;
+    *row = fptr(t);
+    return true;
+  };
+  if (!setting(args[2], &set.temperature, &set.temperature_value) || !setting(args[4], &set.top_p, &set.top_p_value) ||
+      !setting(args[5], &set.min_p, &set.min_p_value) || set.min_p_value > 1.0f)
+    return not_here();
+  if (PyLong_Check(args[3])) {
+    const long long k = PyLong_AsLongLong(args[3]);
+    if (PyErr_Occurred() || k < -0x7fffffffLL || k > 0x7fffffffLL) return not_here();
+    set.top_k_value = (int)k;
+  } else {
+    const at::Tensor* t = nullptr;
+    if (args[3] == Py_None || !optional(args[3], at::kInt, *x, {M}, &t)) return not_here();
+    set.top_k = static_cast<const int*>(ptr(t));
+  }
+  const at::Tensor* given;
+  if (!optional(args[6], at::kInt, *x, {M}, &given)) return not_here();
+  Guard guard(x->device().index());
+  const cudaStream_t s = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  at::Tensor out = given != nullptr ? *given : empty({M}, at::kInt, x->device());
+  if (!succeeded(g_lib.sample(x->const_data_ptr(), M, V, x->stride(0), code, fptr(u), &set,
+                              static_cast<int*>(out.mutable_data_ptr()), s)))
+    return nullptr;
+  return given != nullptr ? Py_NewRef(args[6]) : wrap(std::move(out));
+}
+
 // as_built(module, class): `plain`, for the Python forms, which also take a subclass that keeps the forward.
 PyObject* as_built(PyObject* const* args, Py_ssize_t n) {
   if (n != 2) {
@@ -791,6 +943,10 @@ PyObject* init(PyObject*, PyObject* args) {
   find(&g_lib.attention_block_prefill, "rgk_attention_block_prefill");
   find(&g_lib.mlp_workspace_bytes, "rgk_mlp_workspace_bytes");
   find(&g_lib.residual_channel, "rgk_residual_channel");
+  find(&g_lib.causal_conv, "rgk_causal_conv");
+  find(&g_lib.selective_scan, "rgk_selective_scan");
+  find(&g_lib.selective_scan_workspace_bytes, "rgk_selective_scan_workspace_bytes");
+  find(&g_lib.sample, "rgk_sample");
   if (PyErr_Occurred()) return nullptr;
 #define INTERN(n) if (s_##n == nullptr) s_##n = PyUnicode_InternFromString(#n);
   NAMES(INTERN)
@@ -829,6 +985,9 @@ PyMethodDef methods[] = {
     FAST(prefill),
     FAST(residual_prefill),
     FAST(as_built),
+    FAST(causal_conv),
+    FAST(selective_scan),
+    FAST(sample),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr,
                           nullptr};

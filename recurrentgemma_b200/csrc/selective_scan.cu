@@ -567,6 +567,117 @@ cudaError_t launch(const SelectiveArgs& p, cudaStream_t s) {
   return aligned ? launch_kernel<T, Sh, true>(p, s) : launch_kernel<T, Sh, false>(p, s);
 }
 
+// One time step: the states are read and written once and bound it.  A lane holds four states (8 beyond 128) of each
+// of kRows sequences, L lanes a channel, so that a, d and the bias are read once for kRows sequences and kRows loads of
+// a state are in flight.  kVec: the states' rows are whole vectors of four.
+template <typename T, int S, int L, int kRows, bool kVec>
+__global__ void __launch_bounds__(256)
+selective_step_kernel(const SelectiveArgs p) {
+  const int64_t at = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const int l = threadIdx.x % L;
+  const bool in = at < p.E;
+  const int64_t e = in ? at : p.E - 1;                           // (whole groups of lanes: they shuffle)
+  const int64_t b0 = (int64_t)blockIdx.y * kRows;
+  const int g = (int)(e / p.per_group);
+  auto state_of = [&](int s) { return s / 4 * 4 * L + l * 4 + s % 4; };
+
+  float h[kRows][S], x[kRows], step[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int64_t b = min(b0 + r, p.B - 1);
+    const bool fresh = p.state_in == nullptr || (p.pos != nullptr && pos_is_zero(p.pos, p.pos64, b));
+    const float* from = p.state_in + (b * p.E + e) * p.N;
+#pragma unroll
+    for (int s = 0; s < S; s += 4) {
+      const int n = state_of(s);
+      if (kVec) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (!fresh && n < p.N) v = *reinterpret_cast<const float4*>(from + n);
+        h[r][s] = v.x; h[r][s + 1] = v.y; h[r][s + 2] = v.z; h[r][s + 3] = v.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[r][s + i] = !fresh && n + i < p.N ? from[n + i] : 0.0f;
+      }
+    }
+    x[r] = static_cast<float>(static_cast<const T*>(p.x)[b * p.x_batch + e]);
+    step[r] = static_cast<float>(static_cast<const T*>(p.dt)[b * p.dt_batch + e]);
+  }
+  float a2[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) a2[s] = state_of(s) < p.N ? p.a[e * p.N + state_of(s)] * kLog2e : 0.0f;
+  const float bias = p.dt_bias != nullptr ? p.dt_bias[e] : 0.0f, d = p.d != nullptr ? p.d[e] : 0.0f;
+
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int64_t b = b0 + r;
+    if (b >= p.B) break;
+    const T* vb = static_cast<const T*>(p.b) + b * p.b_batch + (int64_t)g * p.N;
+    const T* vc = static_cast<const T*>(p.c) + b * p.c_batch + (int64_t)g * p.N;
+    float now = step[r] + bias;
+    if (p.softplus) now = softplus_steps(now, now).x;
+    const float put = now * x[r];
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int n = state_of(s);
+      if (n < p.N) {
+        h[r][s] = fmaf(exp2_fast(now * a2[s]), h[r][s], put * static_cast<float>(vb[n]));
+        sum = fmaf(h[r][s], static_cast<float>(vc[n]), sum);
+      }
+    }
+    if (p.state_out != nullptr && in) {
+      float* to = p.state_out + (b * p.E + e) * p.N;
+#pragma unroll
+      for (int s = 0; s < S; s += 4) {
+        const int n = state_of(s);
+        if (kVec) {
+          if (n < p.N) *reinterpret_cast<float4*>(to + n) = make_float4(h[r][s], h[r][s + 1], h[r][s + 2], h[r][s + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (n + i < p.N) to[n + i] = h[r][s + i];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (l == 0 && in) {
+      float out = fmaf(d, x[r], sum);
+      if (p.z != nullptr) {
+        const float z = static_cast<float>(static_cast<const T*>(p.z)[b * p.z_batch + e]);
+        out *= silu_fast(z, z).x;
+      }
+      static_cast<T*>(p.y)[b * p.E + e] = static_cast<T>(out);
+    }
+  }
+}
+
+template <typename T, int S, int L>
+cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
+  const bool vec = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.state_in) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(p.state_out) % 16 == 0;
+  const unsigned across = (unsigned)((p.E + 256 / L - 1) / (256 / L));
+  // four sequences a thread where they still give every SM its threads
+  const bool many = across * p.B >= 4 * 8 * 148;
+  const dim3 grid(across, (unsigned)(many ? (p.B + 3) / 4 : p.B));
+  if (many && vec) selective_step_kernel<T, S, L, 4, true><<<grid, 256, 0, s>>>(p);
+  else if (many) selective_step_kernel<T, S, L, 4, false><<<grid, 256, 0, s>>>(p);
+  else if (vec) selective_step_kernel<T, S, L, 1, true><<<grid, 256, 0, s>>>(p);
+  else selective_step_kernel<T, S, L, 1, false><<<grid, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_step_states(const SelectiveArgs& p, cudaStream_t s) {
+  if (p.N <= 4) return launch_step<T, 4, 1>(p, s);
+  if (p.N <= 8) return launch_step<T, 4, 2>(p, s);
+  if (p.N <= 16) return launch_step<T, 4, 4>(p, s);
+  if (p.N <= 32) return launch_step<T, 4, 8>(p, s);
+  if (p.N <= 64) return launch_step<T, 4, 16>(p, s);
+  if (p.N <= 128) return launch_step<T, 4, 32>(p, s);
+  return launch_step<T, 8, 32>(p, s);
+}
+
 // What a shape takes, relative: `alone` is its time where every CTA has an SM (us for 2048 steps of 16 states), the
 // factor what blocks behind the first round of SMs add; a second CTA on an SM costs half as much as the first.
 double estimate(double alone, int64_t blocks, int sms) {
@@ -619,6 +730,7 @@ cudaError_t launch_selective_scan(SelectiveArgs p, int dtype, cudaStream_t s) {
   if (p.B == 0 || p.E == 0) return cudaSuccess;
   const int size = dtype == 1 ? 2 : 4;
   p.per_group = (int)(p.E / p.groups);
+  if (p.T == 1) return dtype == 1 ? launch_step_states<__nv_bfloat16>(p, s) : launch_step_states<float>(p, s);
   p.copy_x = min(copy_bytes(p.x, p.x_batch, p.x_token, p.per_group, size),
                  copy_bytes(p.dt, p.dt_batch, p.dt_token, p.per_group, size));
   if (p.z != nullptr) p.copy_x = min(p.copy_x, copy_bytes(p.z, p.z_batch, p.z_token, p.per_group, size));

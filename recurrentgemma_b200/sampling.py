@@ -19,7 +19,6 @@ def _per_row(name: str, value, dtype: torch.dtype, logits: torch.Tensor) -> Opti
   return value.contiguous()
 
 
-@torch.no_grad()
 def sample(
     logits: torch.Tensor, uniforms: torch.Tensor,
     temperature: Union[float, torch.Tensor] = 1.0, top_k: Union[int, torch.Tensor] = 0,
@@ -38,6 +37,14 @@ def sample(
   Each setting is a number, or a tensor with one for each row (float32; `top_k` int32).  `uniforms` is
   float32 [...].  The result does not depend on how many rows are drawn together.  V up to 2**20.
   """
+  done = _lib.host().sample(logits, uniforms, temperature, top_k, top_p, min_p, out)
+  if done is not NotImplemented:
+    return done
+  return _sample(logits, uniforms, temperature, top_k, top_p, min_p, out)
+
+
+@torch.no_grad()
+def _sample(logits, uniforms, temperature, top_k, top_p, min_p, out):
   settings = (temperature, top_k, top_p, min_p)
   dev = _lib.require_cuda(logits, uniforms, *(s for s in settings if torch.is_tensor(s)), out)
   v = logits.shape[-1]

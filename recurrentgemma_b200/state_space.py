@@ -46,7 +46,6 @@ def _check_state(state: Optional[torch.Tensor], shape, dtype: torch.dtype) -> No
     raise TypeError(f"the state is {state.dtype}; this operator keeps it in {dtype}")
 
 
-@torch.no_grad()
 def causal_conv(
     x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None, *,
     segment_pos: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
@@ -61,6 +60,14 @@ def causal_conv(
   comes next.  `inplace` overwrites `state` and returns it (a step that a CUDA graph can replay).
   x may be strided over batch and time, as a part of a wider projection is.
   """
+  done = _lib.host().causal_conv(x, w, b, segment_pos, state, activation, return_state, inplace)
+  if done is not NotImplemented:
+    return done
+  return _causal_conv(x, w, b, segment_pos, state, activation, return_state, inplace)
+
+
+@torch.no_grad()
+def _causal_conv(x, w, b, segment_pos, state, activation, return_state, inplace):
   dev = _lib.require_cuda(x, w, b, segment_pos, state)
   dt = _lib.dtype_code(x.dtype)
   assert x.ndim == 3 and w.ndim == 2 and w.shape[1] == x.shape[2], (x.shape, w.shape)
@@ -85,7 +92,6 @@ def causal_conv(
   return y, (new_state if return_state else None)
 
 
-@torch.no_grad()
 def selective_scan(
     x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, *,
     d: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
@@ -104,6 +110,15 @@ def selective_scan(
   start (segment_pos == 0) drops the state in front of it.  `inplace` overwrites `state` and returns it.
   x, dt, z, b and c may be strided over batch and time.
   """
+  done = _lib.host().selective_scan(x, dt, a, b, c, d, z, dt_bias, segment_pos, state, softplus, return_state,
+                                    inplace)
+  if done is not NotImplemented:
+    return done
+  return _selective_scan(x, dt, a, b, c, d, z, dt_bias, segment_pos, state, softplus, return_state, inplace)
+
+
+@torch.no_grad()
+def _selective_scan(x, dt, a, b, c, d, z, dt_bias, segment_pos, state, softplus, return_state, inplace):
   dev = _lib.require_cuda(x, dt, a, b, c, d, z, dt_bias, segment_pos, state)
   code = _lib.dtype_code(x.dtype)
   assert x.ndim == 3 and dt.shape == x.shape and (z is None or z.shape == x.shape), (x.shape, dt.shape)

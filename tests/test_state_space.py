@@ -177,6 +177,9 @@ SCAN = [
     (2, 1, 33, 5, 1, 0, dict(part=True)),
     (4, 1, 64, 128, 2, 0, {}),
     (2, 1, 12, 200, 1, 1, dict(d=False, bias=False)),
+    (70, 1, 2560, 16, 1, 0, {}),
+    (67, 1, 2570, 9, 2, 3, dict(part=True)),
+    (131, 1, 300, 130, 1, 0, dict(z=False)),
     (1, 2, 8, 1, 1, 0, {}),
     (2, 31, 64, 16, 2, 7, {}),
     (2, 32, 36, 16, 1, 0, dict(state=False)),
