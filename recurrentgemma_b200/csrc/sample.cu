@@ -19,6 +19,10 @@
 //
 // Bound: 2 or 4 bytes a token from HBM, and for whole rows and top-p without top-k the 64-bit exponential of every token
 // within 31 temperatures of the maximum (11 double-precision operations, 2 cycles of a scheduler each).
+#include <float.h>
+
+#include <type_traits>
+
 #include "rgk_common.cuh"
 #include "rgk_internal.h"
 #include "tc_common.cuh"
@@ -27,16 +31,16 @@ namespace rgk {
 namespace {
 
 using u64 = unsigned long long;
-#ifndef MINB
-#define MINB 1
-#endif
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;                                       // four to a thread
-constexpr int kList = 2048;                                       // longest list that is sorted, four to a thread
+constexpr int kBins = 2048;
+constexpr int kList = 2048;                                       // longest list that is sorted
+constexpr int kEach = kBins / kThreads;                           // bins, or tokens of a list, to a thread
+static_assert(kList == kBins, "one number a thread for both");
 constexpr int kMostParts = 8;
 constexpr float kRange = 32.0f;                                   // temperatures below the maximum: W = 0 from 31.2 on
 constexpr int kTable = 64;
+constexpr int kStretches = 16;
 
 // The order of the floats as an order of integers (-0 counts as 0, NaN below everything).
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -47,21 +51,18 @@ __device__ __forceinline__ uint32_t key_of(float l) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key);
 }
-constexpr uint32_t kKeyNothing = 0x007fffffu;                     // key of -inf
 
 // 2^F exp((l - max) / T): 2^t with t = n + j / 64 + f, |f| <= 1/128, as 2^n, a table of 2^(j / 64) and the Taylor
-// polynomial of 2^f to degree 4 (4e-14 of the value).
+// polynomial of 2^f to degree 4 (4e-14 of the value).  Of tokens within 44 temperatures of the maximum: the callers
+// drop what it says of others.  No branches: the tokens of a pack are evaluated side by side.
 struct Weights {
   double scale;                                                   // log2(e) / T
   double max;
-  float fmax;
   int bits;                                                       // F
   const double* table;
   __device__ __forceinline__ u64 unit() const { return 1ull << bits; }
   __device__ __forceinline__ u64 operator()(float l) const {
-    if (l == fmax) return unit();
     const double t = ((double)l - max) * scale;
-    if (!(t > -50.0)) return 0;                                   // (NaN too)
     constexpr double kMagic = 105553116266496.0;                  // 1.5 2^46: sums with it are multiples of 1/64
     const double rounded = t + kMagic;
     const int j = __double2loint(rounded);
@@ -77,24 +78,41 @@ struct Weights {
   }
 };
 
-// What is kept: keys above `key`, and those equal to it up to index `last`.
+// What is kept: logits above `end`, and those equal to it up to index `last`.  (NaN is not.)
 struct Cut {
-  uint32_t key;
+  float end;
   int last;
-  __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
+  __device__ __forceinline__ bool keeps(float l, int i) const { return l > end || (l == end && i <= last); }
+};
+// The same as a test for the passes over a row: without ties at the end it is one comparison.
+template <bool kTies> struct Test {
+  Cut cut;
+  __device__ __forceinline__ bool operator()(float l, int i) const { return kTies ? cut.keeps(l, i) : l > cut.end; }
 };
 
-// How a pass sorts tokens into bins: by distance from the maximum (linear, monotonic in the logit), or by key.
+// How a pass sorts tokens into bins: by distance from the maximum (linear, monotonic in the logit; of tokens within
+// kRange temperatures of it), or by key.
 struct Binning {
   bool by_key;
-  float max4, scale4, fmax;                                       // (max - l) / 4, which does not overflow, times 4 bins
+  float max4, scale4;                                             // (max - l) / 4, which does not overflow, times 4 bins
   uint32_t lo, hi;                                                // keys
   int shift;
-  __device__ __forceinline__ int operator()(float l, uint32_t k) const {
-    if (by_key) return k >= lo && k <= hi ? (int)((hi - k) >> shift) : kBins;
-    if (l == fmax) return 0;
-    const float at = fmaf(l, -0.25f, max4) * scale4;
-    return at < (float)kBins ? (int)at : kBins;                   // (NaN is in none)
+  __device__ __forceinline__ int operator()(float l) const {
+    if (by_key) {
+      const uint32_t k = key_of(l);
+      return k >= lo && k <= hi ? (int)((hi - k) >> shift) : kBins;
+    }
+    // (rounded down by the sum with 2^23)
+    return min((int)(__float_as_uint(__fadd_rd(fmaf(l, -0.25f, max4) * scale4, 8388608.0f)) & 0xffffu), kBins - 1);
+  }
+  // The smallest logit that `was` may keep whose bin is at most `bin`, by halving the keys below the maximum.
+  __device__ float smallest(int bin, const Cut& was, float largest) const {
+    uint32_t out = key_of(was.end) - (was.last >= 0), in = key_of(largest);  // (the maximum is in bin 0)
+    while (in - out > 1) {
+      const uint32_t mid = out + (in - out) / 2;
+      if ((*this)(value_of(mid)) <= bin) in = mid; else out = mid;
+    }
+    return value_of(in);
   }
 };
 
@@ -112,19 +130,19 @@ struct Shared {
       u64 all_weight[kBins];
     };
     struct {
-      u64 order[kList];                                           // list: in the first CTA
-      u64 kept[kList];
-      float value[kList];
-      int index[kList];
+      u64 order[kList], kept[kList];                              // the list: in the first CTA
     };
   };
   double table[kTable];
-  u64 part[kWarps + 1];
+  u64 part[kWarps];
+  u64 stretch[kWarps][kStretches];                                // sums of the pieces of a warp's run
   u64 total[kMostParts];                                          // one from each CTA of the cluster
   float best[kMostParts];
   int best_at[kMostParts];
   unsigned key_lo[kMostParts], key_hi[kMostParts];
   Found found;
+  unsigned length;                                                // of the list
+  unsigned mine, place;                                           // of it in this CTA: how many, and from where on
   int walked;                                                     // an index that a warp of the cluster has found
 };
 
@@ -134,9 +152,9 @@ template <typename P> __device__ __forceinline__ P* peer(P* p, int rank) {
   return r;
 }
 
-// A row's CTAs, and the calling warp's run of it in 16-byte packs.
+// A row's CTAs, and the calling warp's run of it in packs of four tokens.
+constexpr int kPer = 4, kAhead = 4;                               // packs that a lane asks for at a time
 template <typename T> struct Row {
-  static constexpr int kPer = 16 / (int)sizeof(T);
   const T* row;                                                   // its first token
   int V, head;                                                    // tokens in front of it in its first pack
   int parts, rank;
@@ -144,32 +162,56 @@ template <typename T> struct Row {
   __device__ __forceinline__ void sync() const {
     if (parts > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
   }
-  // fn(values, first index, ...) of every pack, all lanes together; what does not exist is NaN
-  template <typename F> __device__ __forceinline__ void each(F&& fn) const {
-    const int lane = threadIdx.x & 31;
-    for (int g0 = begin; g0 < end; g0 += 128) {
-      uint4 raw[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = (g0 + 32 * u + lane) * kPer - head;
-        if (i >= 0 && i + kPer <= V && g0 + 32 * u + lane < end) raw[u] = *reinterpret_cast<const uint4*>(row + i);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (g0 + 32 * u >= end) break;
-        const bool mine = g0 + 32 * u + lane < end;
-        const int i = (g0 + 32 * u + lane) * kPer - head;
-        float v[kPer];
-        if (mine && i >= 0 && i + kPer <= V) {
-          unpack<T>(raw[u], v);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) v[j] = mine && i + j >= 0 && i + j < V ? static_cast<float>(row[i + j]) : NAN;
-        }
-        if (fn(v, i)) return;
-      }
+  using Raw = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+  __device__ __forceinline__ bool whole(int g) const { return g < end && g * kPer >= head && (g + 1) * kPer - head <= V; }
+  static __device__ __forceinline__ void unpack4(const Raw& raw, float (&v)[kPer]) {
+    if constexpr (sizeof(T) == 4) {
+      unpack<T>(raw, v);
+    } else {
+      v[0] = bf16_lo(raw.x); v[1] = bf16_hi(raw.x); v[2] = bf16_lo(raw.y); v[3] = bf16_hi(raw.y);
     }
   }
+  __device__ __forceinline__ void widen(const Raw& raw, int g, float (&v)[kPer]) const {
+    if (whole(g)) {
+      unpack4(raw, v);
+    } else {
+      const int i = g * kPer - head;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[j] = g < end && i + j >= 0 && i + j < V ? static_cast<float>(row[i + j]) : NAN;
+    }
+  }
+  // fn(values, first index) of every pack, all lanes together; what does not exist is NaN.  Packs are taken 32 kAhead
+  // at a time, after which done(the first of them) is called.
+  template <typename F, typename G> __device__ __forceinline__ void each(F&& fn, G&& done) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int g0 = begin; g0 < end; g0 += 32 * kAhead) {
+      const int g = g0 + lane;
+      const T* at = row + ((int64_t)g * kPer - head);
+      Raw raw[kAhead];
+      if (g0 * kPer >= head && g0 + 32 * kAhead <= end && (g0 + 32 * kAhead) * kPer - head <= V) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) raw[u] = *reinterpret_cast<const Raw*>(at + 32 * u * kPer);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          float v[kPer];
+          unpack4(raw[u], v);
+          fn(v, (g + 32 * u) * kPer - head);
+        }
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < kAhead; ++u) {
+          raw[0] = {};
+          if (whole(g + 32 * u)) raw[0] = *reinterpret_cast<const Raw*>(at + 32 * u * kPer);
+          float v[kPer];
+          widen(raw[0], g + 32 * u, v);
+          fn(v, (g + 32 * u) * kPer - head);
+        }
+      }
+      done(g0);
+    }
+  }
+  template <typename F> __device__ __forceinline__ void each(F&& fn) const { each(fn, [](int) {}); }
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -231,40 +273,55 @@ __device__ __forceinline__ u64 cluster_before(u64 v, const Row<T>& row, Shared& 
 // The first index at which the running sum of weight(l, i) exceeds `target(total)`, for all of the cluster.
 template <typename T, typename F, typename G>
 __device__ int walk(const Row<T>& row, Shared& sh, F&& weight, G&& target) {
-  const int lane = threadIdx.x & 31;
-  u64 mine = 0;
-  row.each([&](const float (&v)[Row<T>::kPer], int i) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // every lane's sums, stretch after stretch of the run, so that the last stage reads one stretch again and no more
+  u64 mine = 0, stretch = 0;
+  const int per = (row.end - row.begin + 32 * kAhead * kStretches - 1) / (32 * kAhead * kStretches) * 32 * kAhead;
+  row.each([&](const float (&v)[kPer], int i) {
 #pragma unroll
-    for (int j = 0; j < Row<T>::kPer; ++j) mine += weight(v[j], i + j);
-    return false;
+    for (int j = 0; j < kPer; ++j) stretch += weight(v[j], i + j);
+  }, [&](int g0) {
+    const int behind = g0 + 32 * kAhead - row.begin;
+    if (behind % per == 0 || g0 + 32 * kAhead >= row.end) {
+      stretch = warp_sum(stretch);
+      if (lane == 0) sh.stretch[warp][(behind - 1) / per] = stretch;
+      mine += stretch;
+      stretch = 0;
+    }
   });
-  mine = warp_sum(mine);
   u64 total;
   u64 before = cluster_before(mine, row, sh, &total);
   const u64 limit = target(total);
   if (before <= limit && before + mine > limit) {                 // one warp of the cluster
-    row.each([&](const float (&v)[Row<T>::kPer], int i) {
-      u64 w[Row<T>::kPer], sum = 0;
+    int at = 0;
+    while (at + 1 < kStretches && before + sh.stretch[warp][at] <= limit) before += sh.stretch[warp][at++];
+    for (int g0 = row.begin + at * per; g0 < row.end; g0 += 32) {
+      const int g = g0 + lane, i = g * kPer - row.head;
+      typename Row<T>::Raw raw = {};
+      if (row.whole(g)) raw = *reinterpret_cast<const typename Row<T>::Raw*>(row.row + i);
+      float v[kPer];
+      row.widen(raw, g, v);
+      u64 w[kPer], sum = 0;
 #pragma unroll
-      for (int j = 0; j < Row<T>::kPer; ++j) sum += w[j] = weight(v[j], i + j);
+      for (int j = 0; j < kPer; ++j) sum += w[j] = weight(v[j], i + j);
       const u64 upto = before + warp_upto(sum);
       const unsigned over = __ballot_sync(0xffffffffu, upto > limit);
       if (over == 0) {
         before = __shfl_sync(0xffffffffu, upto, 31);
-        return false;
+        continue;
       }
       if (lane == __ffs(over) - 1) {
-        u64 at = upto - sum;
+        u64 sofar = upto - sum;
         int found = i;
 #pragma unroll
-        for (int j = 0; j < Row<T>::kPer; ++j) {
-          if (at <= limit) found = i + j;
-          at += w[j];
+        for (int j = 0; j < kPer; ++j) {
+          if (sofar <= limit) found = i + j;
+          sofar += w[j];
         }
         for (int r = 0; r < row.parts; ++r) peer(&sh, r)->walked = found;
       }
-      return true;
-    });
+      break;
+    }
   }
   row.sync();
   return sh.walked;
@@ -279,33 +336,40 @@ __device__ Found histogram(const Row<T>& row, Shared& sh, const Binning& bins, c
   __syncthreads();
   for (int i = tid; i < kBins; i += kThreads) sh.count[i] = sh.lo[i] = sh.hi[i] = 0;
   __syncthreads();
-  row.each([&](const float (&v)[Row<T>::kPer], int i) {
+  row.each([&](const float (&v)[kPer], int i) {
 #pragma unroll
-    for (int j = 0; j < Row<T>::kPer; ++j) {
-      const uint32_t k = key_of(v[j]);
-      const int bin = bins(v[j], k);
-      if (bin >= kBins || !eligible(k, i + j)) continue;
+    for (int j = 0; j < kPer; ++j) {
+      const int bin = bins(v[j]);
+      const u64 w = kCount ? 0ull : weight(v[j]);
+      if (bin >= kBins || !eligible(v[j], i + j)) continue;
       atomicAdd(&sh.count[bin], 1u);
       if (!kCount) {
-        const u64 w = weight(v[j]);
         const unsigned lo = (unsigned)w;
         const unsigned carry = atomicAdd(&sh.lo[bin], lo) + lo < lo;
         const unsigned hi = (unsigned)(w >> 32) + carry;
         if (hi != 0) atomicAdd(&sh.hi[bin], hi);
       }
     }
-    return false;
   });
   row.sync();
   {                                                               // every CTA adds up its share of the bins
     const int each = kBins / row.parts;
     for (int i = row.rank * each + tid; i < (row.rank + 1) * each; i += kThreads) {
-      unsigned count = 0;
+      unsigned counts[kMostParts], los[kMostParts], his[kMostParts], count = 0;
       u64 w = 0;
-      for (int r = 0; r < row.parts; ++r) {
-        const Shared* s = row.parts > 1 ? peer(&sh, r) : &sh;
-        count += s->count[i];
-        if (!kCount) w += ((u64)s->hi[i] << 32) + s->lo[i];
+#pragma unroll
+      for (int r = 0; r < kMostParts; ++r) {                      // (asked for all at once)
+        counts[r] = los[r] = his[r] = 0;
+        if (r < row.parts) {
+          const Shared* s = peer(&sh, r);
+          counts[r] = s->count[i];
+          if (!kCount) { los[r] = s->lo[i]; his[r] = s->hi[i]; }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kMostParts; ++r) {
+        count += counts[r];
+        w += ((u64)his[r] << 32) + los[r];
       }
       Shared* first = row.parts > 1 ? peer(&sh, 0) : &sh;
       first->all_count[i] = count;
@@ -314,11 +378,11 @@ __device__ Found histogram(const Row<T>& row, Shared& sh, const Binning& bins, c
   }
   row.sync();
   if (row.rank == 0) {
-    u64 mine[4], sum = 0, counts = 0, total, all;
+    u64 mine[kEach], sum = 0, counts = 0, total, all;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      sum += mine[j] = sh.all_weight[tid * 4 + j];
-      counts += sh.all_count[tid * 4 + j];
+    for (int j = 0; j < kEach; ++j) {
+      sum += mine[j] = sh.all_weight[tid * kEach + j];
+      counts += sh.all_count[tid * kEach + j];
     }
     u64 before = block_before(sum, sh, &total), upto = block_before(counts, sh, &all);
     if (share >= 0.0) target = max(1ull, (u64)ceil(share * (double)total));
@@ -328,11 +392,11 @@ __device__ Found histogram(const Row<T>& row, Shared& sh, const Binning& bins, c
     }
     if (before < target && before + sum >= target) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned n = sh.all_count[tid * 4 + j];
+      for (int j = 0; j < kEach; ++j) {
+        const unsigned n = sh.all_count[tid * kEach + j];
         upto += n;
         if (before < target && before + mine[j] >= target) {
-          f.bin = tid * 4 + j;
+          f.bin = tid * kEach + j;
           f.in_bin = n;
           f.upto = (unsigned)upto;
           f.above = before;
@@ -348,70 +412,80 @@ __device__ Found histogram(const Row<T>& row, Shared& sh, const Binning& bins, c
   return f;
 }
 
-// Brings the tokens that `wanted` picks, 2048 at most, together in the first CTA, in the order of their indices.
+// Brings the tokens that `wanted` picks, 2048 at most, together in the first CTA, in any order, as sort_list's words:
+// in each CTA first (in `kept`), then with one place for all of a CTA's in the first one's `order`.
 template <typename T, typename F>
 __device__ int gather(const Row<T>& row, Shared& sh, F&& wanted) {
-  u64 mine = 0;
-  row.each([&](const float (&v)[Row<T>::kPer], int i) {
+  if (threadIdx.x == 0) sh.mine = sh.length = 0;
+  row.sync();
+  row.each([&](const float (&v)[kPer], int i) {
+    bool any = false;
 #pragma unroll
-    for (int j = 0; j < Row<T>::kPer; ++j) mine += wanted(v[j], i + j);
-    return false;
-  });
-  mine = warp_sum(mine);
-  u64 total;
-  unsigned at = (unsigned)cluster_before(mine, row, sh, &total);
-  Shared* first = row.parts > 1 ? peer(&sh, 0) : &sh;
-  if (mine != 0) {
-    row.each([&](const float (&v)[Row<T>::kPer], int i) {
-      unsigned picked = 0;
+    for (int j = 0; j < kPer; ++j) any |= wanted(v[j], i + j);
+    if (any) {
 #pragma unroll
-      for (int j = 0; j < Row<T>::kPer; ++j) picked |= (unsigned)wanted(v[j], i + j) << j;
-      if (__any_sync(0xffffffffu, picked != 0)) {
-        const unsigned n = __popc(picked), upto = (unsigned)warp_upto(n);
-        unsigned to = at + upto - n;
-#pragma unroll
-        for (int j = 0; j < Row<T>::kPer; ++j) {
-          if (((picked >> j) & 1u) && to < kList) {
-            first->value[to] = v[j];
-            first->index[to] = i + j;
-            ++to;
-          }
-        }
-        at += __shfl_sync(0xffffffffu, upto, 31);
+      for (int j = 0; j < kPer; ++j) {
+        if (!wanted(v[j], i + j)) continue;
+        const unsigned to = atomicAdd(&sh.mine, 1u);
+        if (to < kList) sh.kept[to] = (u64)~key_of(v[j]) << 32 | (unsigned)(i + j);
       }
-      return false;
-    });
+    }
+  });
+  __syncthreads();
+  const unsigned n = min(sh.mine, (unsigned)kList);
+  Shared* first = row.parts > 1 ? peer(&sh, 0) : &sh;
+  if (threadIdx.x == 0) sh.place = atomicAdd(&first->length, n);
+  __syncthreads();
+  for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+    if (sh.place + i < kList) first->order[sh.place + i] = sh.kept[i];
   }
   row.sync();
-  return (int)min(total, (u64)kList);
+  return min(sh.length, (unsigned)kList);                         // (of use in the first CTA)
 }
 
-// order[] = places in the list by key descending, then by place; padded to a power of two, which it returns.
-__device__ int sort_list(Shared& sh, int n) {
-  int size = 32;
+// Sorts the first n words of `words`, which are all different, ascending: short lists by counting what is smaller, long
+// ones by exchanges, those over less than 64 places within a warp's own.
+__device__ void sort_list(u64* words, int n) {
+  if (n <= 256) {
+    const u64 mine = threadIdx.x < n ? words[threadIdx.x] : ~0ull;
+    int place = 0;
+    if (threadIdx.x < n) {
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) place += words[i] < mine;
+    }
+    __syncthreads();
+    if (threadIdx.x < n) words[place] = mine;
+    __syncthreads();
+    return;
+  }
+  int size = 512;
   while (size < n) size <<= 1;
-  for (int i = threadIdx.x; i < size; i += kThreads)
-    sh.order[i] = i < n ? (u64)~key_of(sh.value[i]) << 32 | (unsigned)i : ~0ull;
+  for (int i = n + threadIdx.x; i < size; i += kThreads) words[i] = ~0ull;
+  __syncthreads();
+  bool wide = false;
   for (int k = 2; k <= size; k <<= 1) {
     for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
+      if (j >= 64 || wide) __syncthreads(); else __syncwarp();
+      wide = j >= 64;
+#pragma unroll 2
       for (int i = threadIdx.x; i < size / 2; i += kThreads) {
         const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const u64 x = sh.order[a], y = sh.order[b];
-        if ((x > y) == ((a & k) == 0)) { sh.order[a] = y; sh.order[b] = x; }
+        const u64 x = words[a], y = words[b];
+        if ((x > y) == ((a & k) == 0)) { words[a] = y; words[b] = x; }
       }
     }
   }
   __syncthreads();
-  return size;
 }
+// Of a list's word: the logit, descending in the order of the words, and the index.
+__device__ __forceinline__ float logit_of(u64 word) { return value_of(~(uint32_t)(word >> 32)); }
 
-// The first place at which the running sum of four values a thread reaches `target` (sum >= target), for the whole CTA.
-__device__ __forceinline__ int first_reaching(const u64 (&v)[4], u64 before, u64 target, Shared& sh) {
+// The first place at which the running sum of kEach values a thread reaches `target` (sum >= target), for the whole CTA.
+__device__ __forceinline__ int first_reaching(const u64 (&v)[kEach], u64 before, u64 target, Shared& sh) {
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (before < target && before + v[j] >= target) sh.walked = threadIdx.x * 4 + j;
+  for (int j = 0; j < kEach; ++j) {
+    if (before < target && before + v[j] >= target) sh.walked = threadIdx.x * kEach + j;
     before += v[j];
   }
   __syncthreads();
@@ -433,68 +507,61 @@ struct Settings {
 // The token, from a list that holds every token that can be kept.  wanted: what top-p has to reach, where top-k does not
 // come before it.
 __device__ int finish_list(Shared& sh, int n, const Weights& weight, const Settings& set, u64 wanted) {
-  const int tid = threadIdx.x;
-  sort_list(sh, n);
-  u64 w[4], sum = 0, total, before;
-  const int first = tid * 4, longest = set.top_k > 0 ? min(n, set.top_k) : n;
+  const int tid = threadIdx.x, first = tid * kEach, longest = set.top_k > 0 ? min(n, set.top_k) : n;
+  sort_list(sh.order, n);
+  u64 w[kEach], sum = 0, total, before;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    w[j] = first + j < longest ? weight(sh.value[(unsigned)sh.order[first + j]]) : 0ull;
-    sum += w[j];
-  }
+  for (int j = 0; j < kEach; ++j) sum += w[j] = first + j < longest ? weight(logit_of(sh.order[first + j])) : 0ull;
   before = block_before(sum, sh, &total);
   int length = longest;
   if (set.top_p < 1.0f) {
     if (set.top_k > 0) wanted = max(1ull, (u64)ceil((double)set.top_p * (double)total));
     if (wanted <= total) length = min(length, first_reaching(w, before, wanted, sh) + 1);
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (first + j < n) sh.kept[(unsigned)sh.order[first + j]] = first + j < length && w[j] >= set.least ? w[j] : 0ull;
-  }
+  // those that are kept by index, each with its place in the list
+  for (int i = tid; i < length; i += kThreads) sh.kept[i] = sh.order[i] << 32 | (unsigned)i;
   __syncthreads();
+  sort_list(sh.kept, length);
   sum = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) sum += w[j] = first + j < n ? sh.kept[first + j] : 0ull;
+  for (int j = 0; j < kEach; ++j) {
+    w[j] = first + j < length ? weight(logit_of(sh.order[(unsigned)sh.kept[first + j]])) : 0ull;
+    sum += w[j] = w[j] >= set.least ? w[j] : 0ull;
+  }
   before = block_before(sum, sh, &total);
-  return sh.index[first_reaching(w, before, set.limit(total) + 1, sh)];
+  return (int)(sh.kept[first_reaching(w, before, set.limit(total) + 1, sh)] >> 32);
 }
 
 // The shortest prefix of what `was` keeps with `target` tokens, or with `share` of the weight.  True: it, and everything
 // in front of it, is in a list of `*n` tokens, where `*wanted` is to be reached; else *cut is its end.
-template <bool kCount, typename T>
-__device__ bool prefix(const Row<T>& row, Shared& sh, const Weights& weight, Binning bins, const Cut& was, double share,
+template <bool kCount, bool kTies, typename T>
+__device__ bool prefix(const Row<T>& row, Shared& sh, const Weights& weight, Binning bins, float largest, const Cut was, double share,
                        u64 target, Cut* cut, int* n, u64* wanted) {
   *cut = was;
-  auto eligible = [&](uint32_t k, int i) { return was.keeps(k, i); };
+  const Test<kTies> eligible{was};
   Found f = histogram<kCount>(row, sh, bins, weight, eligible, share, target);
   if (f.bin < 0) return false;                                    // all of it
   *wanted = f.target;
-  auto upto = [&](float l, int i) {
-    const uint32_t k = key_of(l);
-    return bins(l, k) <= f.bin && f.bin < kBins && eligible(k, i);
-  };
-  auto within = [&](float l, int i) {
-    const uint32_t k = key_of(l);
-    return bins(l, k) == f.bin && eligible(k, i);
-  };
+  // the bin as a range of logits: from `least` to below `above`
+  float least = bins.smallest(f.bin, was, largest);
   if (f.upto <= kList) {
-    *n = gather(row, sh, upto);
+    *n = gather(row, sh, [&](float l, int i) { return l >= least && eligible(l, i); });
     return true;
   }
+  float above = f.bin > 0 ? bins.smallest(f.bin - 1, was, largest) : INFINITY;
+  auto within = [&](float l, int i) { return l >= least && l < above && eligible(l, i); };
   u64 left = f.target - f.above;                                  // to be reached within the bin
   while (f.in_bin > kList) {
     uint32_t lo = ~0u, hi = 0;
-    row.each([&](const float (&v)[Row<T>::kPer], int i) {
+    row.each([&](const float (&v)[kPer], int i) {
 #pragma unroll
-      for (int j = 0; j < Row<T>::kPer; ++j) {
+      for (int j = 0; j < kPer; ++j) {
         if (within(v[j], i + j)) {
           const uint32_t k = key_of(v[j]);
           lo = min(lo, k);
           hi = max(hi, k);
         }
       }
-      return false;
     });
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
@@ -512,9 +579,9 @@ __device__ bool prefix(const Row<T>& row, Shared& sh, const Weights& weight, Bin
     if (lo == hi) {                                               // ties: the first of them, by counting
       const u64 w = kCount ? 1ull : weight(value_of(lo));
       const u64 ties = (left + w - 1) / w;
-      cut->key = lo;
+      cut->end = value_of(lo);
       cut->last = ties >= f.in_bin ? row.V : walk(row, sh, [&](float l, int i) -> u64 {
-        return key_of(l) == lo && eligible(lo, i);
+        return l == cut->end && eligible(l, i);
       }, [&](u64) { return ties - 1; });
       return false;
     }
@@ -524,23 +591,26 @@ __device__ bool prefix(const Row<T>& row, Shared& sh, const Weights& weight, Bin
     bins.shift = max(0, 32 - __clz(hi - lo) - 11);
     f = histogram<kCount>(row, sh, bins, weight, eligible, -1.0, left);
     left -= f.above;
+    const uint32_t from = hi - ((uint32_t)f.bin << bins.shift);   // the bin's largest key
+    least = value_of(max(lo, from - ((1u << bins.shift) - 1)));
+    above = value_of(from + 1);
   }
   *n = gather(row, sh, within);
   if (row.rank == 0) {
-    sort_list(sh, *n);
-    u64 w[4], sum = 0, total;
+    sort_list(sh.order, *n);
+    u64 w[kEach], sum = 0, total;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = threadIdx.x * 4 + j;
-      sum += w[j] = at >= *n ? 0ull : kCount ? 1ull : weight(sh.value[(unsigned)sh.order[at]]);
+    for (int j = 0; j < kEach; ++j) {
+      const int at = threadIdx.x * kEach + j;
+      sum += w[j] = at >= *n ? 0ull : kCount ? 1ull : weight(logit_of(sh.order[at]));
     }
     const u64 before = block_before(sum, sh, &total);
-    const int at = (unsigned)sh.order[first_reaching(w, before, left, sh)];
-    const Found end{sh.index[at], key_of(sh.value[at]), 0, 0, 0};
+    const u64 last = sh.order[first_reaching(w, before, left, sh)];
+    const Found end{(int)(unsigned)last, ~(uint32_t)(last >> 32), 0, 0, 0};
     if ((int)threadIdx.x < row.parts) peer(&sh, threadIdx.x)->found = end;
   }
   row.sync();
-  cut->key = sh.found.in_bin;
+  cut->end = value_of(sh.found.in_bin);
   cut->last = sh.found.bin;
   row.sync();
   return false;
@@ -549,7 +619,7 @@ __device__ bool prefix(const Row<T>& row, Shared& sh, const Weights& weight, Bin
 template <typename V> __device__ __forceinline__ V setting(const V* p, V value, int64_t m) { return p != nullptr ? p[m] : value; }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, MINB)
+__global__ void __launch_bounds__(kThreads, 2)
 sample_kernel(const SampleArgs p, int parts) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
@@ -558,11 +628,11 @@ sample_kernel(const SampleArgs p, int parts) {
   Row<T> row;
   row.row = static_cast<const T*>(p.logits) + m * p.row_stride;
   row.V = (int)p.V;
-  row.head = (int)((reinterpret_cast<uintptr_t>(row.row) & 15u) / sizeof(T));
+  row.head = (int)(reinterpret_cast<uintptr_t>(row.row) / sizeof(T) % kPer);
   row.parts = parts;
   row.rank = (int)(blockIdx.x - m * parts);
-  const int packs = (row.head + row.V + Row<T>::kPer - 1) / Row<T>::kPer;
-  const int run = ((packs + parts * kWarps - 1) / (parts * kWarps) + 31) & ~31;
+  const int packs = (row.head + row.V + kPer - 1) / kPer;
+  const int run = (packs + parts * kWarps - 1) / (parts * kWarps);
   row.begin = min(packs, (row.rank * kWarps + warp) * run);
   row.end = min(packs, row.begin + run);
   if (parts > 1) cluster_arrive();                                // "this CTA runs"
@@ -571,12 +641,11 @@ sample_kernel(const SampleArgs p, int parts) {
   // the first maximum
   float best = -INFINITY;
   int at = row.V;
-  row.each([&](const float (&v)[Row<T>::kPer], int i) {
+  row.each([&](const float (&v)[kPer], int i) {
 #pragma unroll
-    for (int j = 0; j < Row<T>::kPer; ++j) {
+    for (int j = 0; j < kPer; ++j) {
       if (v[j] > best) { best = v[j]; at = i + j; }
     }
-    return false;
   });
   auto better = [&](float ob, int oa) {
     if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
@@ -584,10 +653,10 @@ sample_kernel(const SampleArgs p, int parts) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
   if (lane == 0) {
-    sh.kept[warp] = (u64)__float_as_uint(best) << 32 | (unsigned)at;
+    sh.part[warp] = (u64)__float_as_uint(best) << 32 | (unsigned)at;
   }
   __syncthreads();
-  for (int w = 0; w < kWarps; ++w) better(__uint_as_float((unsigned)(sh.kept[w] >> 32)), (int)(unsigned)sh.kept[w]);
+  for (int w = 0; w < kWarps; ++w) better(__uint_as_float((unsigned)(sh.part[w] >> 32)), (int)(unsigned)sh.part[w]);
   if (parts > 1) cluster_wait();
   if (tid < parts) {
     peer(&sh, tid)->best[row.rank] = best;
@@ -602,7 +671,7 @@ sample_kernel(const SampleArgs p, int parts) {
     return;                                                       // (nothing remote is under way)
   }
   best += 0.0f;
-  const Weights weight{1.4426950408889634 / (double)temperature, (double)best, best, p.bits, sh.table};
+  const Weights weight{1.4426950408889634 / (double)temperature, (double)best, p.bits, sh.table};
   Settings set;
   set.top_k = setting(p.top_k, p.top_k_value, m);
   if (set.top_k < 0 || set.top_k >= row.V) set.top_k = 0;
@@ -610,24 +679,39 @@ sample_kernel(const SampleArgs p, int parts) {
   const double min_p = (double)setting(p.min_p, p.min_p_value, m);
   set.least = min_p > 0.0 ? (u64)ceil(fmin(min_p, 1.0) * (double)weight.unit()) : 0ull;
   set.uniform = p.uniforms[m];
-  const Binning bins{false, 0.25f * best, 4.0f * kBins / kRange / temperature, best, 0, 0, 0};
+  const Binning bins{false, 0.25f * best, fminf(4.0f * kBins / kRange / temperature, FLT_MAX), 0, 0, 0};
 
-  Cut cut{kKeyNothing, row.V};                                    // all but -inf and NaN
+  if (best == INFINITY) {                                         // they share evenly, nothing else weighs anything
+    const int token = walk(row, sh, [&](float l, int) -> u64 { return l == INFINITY; }, [&](u64 total) {
+      u64 kept = set.top_k > 0 ? min(total, (u64)set.top_k) : total;
+      if (set.top_p < 1.0f) kept = min(kept, max(1ull, (u64)ceil((double)set.top_p * (double)kept)));
+      return set.limit(kept);
+    });
+    if (row.rank == 0 && tid == 0) p.out[m] = token;
+    return;
+  }
+
+  // all but NaN, -inf and what weighs nothing
+  Cut cut{__fmaf_rd(-kRange, temperature, best), -1};
   int n = 0;
   u64 wanted = 0;
   bool listed = false;
-  if (set.top_k > 0) listed = prefix<true>(row, sh, weight, bins, cut, -1.0, (u64)set.top_k, &cut, &n, &wanted);
+  if (set.top_k > 0) listed = prefix<true, false>(row, sh, weight, bins, best, cut, -1.0, (u64)set.top_k, &cut, &n, &wanted);
   if (!listed && set.top_p < 1.0f) {
     set.top_k = 0;                                                // (in the cut by now)
-    listed = prefix<false>(row, sh, weight, bins, cut, fmax((double)set.top_p, 0.0), 0, &cut, &n, &wanted);
+    const double share = fmax((double)set.top_p, 0.0);
+    listed = cut.last < 0 ? prefix<false, false>(row, sh, weight, bins, best, cut, share, 0, &cut, &n, &wanted)
+                          : prefix<false, true>(row, sh, weight, bins, best, cut, share, 0, &cut, &n, &wanted);
   }
   int token = 0;
   if (!listed) {
-    token = walk(row, sh, [&](float l, int i) -> u64 {
-      if (!cut.keeps(key_of(l), i)) return 0;
-      const u64 w = weight(l);
-      return w >= set.least ? w : 0;
-    }, [&](u64 total) { return set.limit(total); });
+    auto draw = [&](auto keeps) {
+      return walk(row, sh, [&](float l, int i) -> u64 {
+        const u64 w = weight(l);
+        return keeps(l, i) && w >= set.least ? w : 0ull;
+      }, [&](u64 total) { return set.limit(total); });
+    };
+    token = cut.last < 0 ? draw(Test<false>{cut}) : draw(Test<true>{cut});
   } else if (row.rank == 0) {
     token = finish_list(sh, n, weight, set, wanted);
   }
@@ -646,9 +730,11 @@ cudaError_t launch_sample(const SampleArgs& p, int dtype, cudaStream_t s) {
     return cudaFuncSetAttribute(sample_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
   }, &sms);
   if (e != cudaSuccess) return e;
-  // CTAs of a row: as long as each has 4096 tokens and they do not fill the device twice
+  // CTAs of a row: as many as are on the device at a time, each with 4096 tokens at least.  A CTA more costs a row its
+  // barriers and its share of the merging; 256000 tokens with 1, 2, 4 and 8 of them: top-p on 256 rows 359 / 387 / 426 /
+  // 567 us, on 64 rows 209 / 125 / 110 / 149, on 16 rows 208 / 125 / 79 / 74, on one row 199 / 117 / 72 / 52.
   int parts = kMostParts;
-  while (parts > 1 && (p.V < parts * 4096 || p.M * parts > 4 * sms)) parts /= 2;
+  while (parts > 1 && (p.V < parts * 4096 || p.M * parts > 2 * sms)) parts /= 2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)parts;
