@@ -22,6 +22,7 @@
 // works on a fifth CTA while others have four (1090 -> 1023 us in the form with one team); a state goes from chunk to chunk through state_out.
 #include <type_traits>
 
+#include "packed.cuh"
 #include "rgk_common.cuh"
 #include "rgk_internal.h"
 
@@ -31,42 +32,6 @@ namespace {
 constexpr int kTeam = 128;                                        // threads of each half of a CTA
 constexpr int kMostBlocks = 1 << 16;                             // whose progress the workspace has room for
 constexpr unsigned kWaitLimit = 1u << 23;                       // polls, 0.2 us and more each
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float exp2_fast(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
-// Two float32 operations in one instruction, on pairs as they lie in memory: half the issue slots of the same work
-// (the multiply-add pipe itself takes as long for a pair as for two).
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float lo, float hi) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 split(Pair v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
-__device__ __forceinline__ Pair exp2_pair(Pair x) {
-  const float2 v = split(x);
-  return pair(exp2_fast(v.x), exp2_fast(v.y));
-}
 
 // softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1]: log1p(e) / e by a polynomial fitted for the
 // smallest largest relative error on [0, 1] (5e-9; 1.8e-7 in float32 arithmetic).  Steps of 1e-3 come out with their
@@ -81,14 +46,6 @@ __device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
 #pragma unroll
   for (int i = 8; i >= 0; --i) p = fma2(p, e, pair(k[i], k[i]));
   return split(fma2(p, e, pair(fmaxf(v0, 0.0f), fmaxf(v1, 0.0f))));
-}
-
-__device__ __forceinline__ float2 silu_fast(float v0, float v1) {
-  const float2 arg = split(mul2(pair(v0, v1), pair(-kLog2e, -kLog2e)));
-  float r0, r1;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(1.0f + exp2_fast(arg.x)));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(1.0f + exp2_fast(arg.y)));
-  return split(mul2(pair(v0, v1), pair(r0, r1)));
 }
 
 // four consecutive elements, at an address aligned to four of them
