@@ -525,74 +525,113 @@ cudaError_t launch(const SelectiveArgs& p, cudaStream_t s) {
 }
 
 // One time step: the states are read and written once and bound it.  A lane holds four states (8 beyond 128) of each
-// of kRows sequences, L lanes a channel, so that a, d and the bias are read once for kRows sequences and kRows loads of
-// a state are in flight.  kVec: the states' rows are whole vectors of four.
+// of kRows sequences, L lanes a channel, so that a, d and the bias are read once for kRows sequences and all that is
+// read of kRows sequences is in flight at a time.  kVec: states, b and c are read and written four at a time.  256 x 5120
+// x 16 in bfloat16: STEP_TIME.
+template <typename T> struct Four;                               // four elements as they lie in memory
+template <> struct Four<float> { using type = float4; };
+template <> struct Four<__nv_bfloat16> { using type = uint2; };
+__device__ __forceinline__ void widen4(const float4& v, float* f) { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+__device__ __forceinline__ void widen4(const uint2& v, float* f) {
+  f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
+}
+
 template <typename T, int S, int L, int kRows, bool kVec>
 __global__ void __launch_bounds__(256)
 selective_step_kernel(const SelectiveArgs p) {
+  using Raw = typename Four<T>::type;
+  constexpr int Q = S / 4;
   const int64_t at = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
   const int l = threadIdx.x % L;
   const bool in = at < p.E;
   const int64_t e = in ? at : p.E - 1;                           // (whole groups of lanes: they shuffle)
   const int64_t b0 = (int64_t)blockIdx.y * kRows;
   const int g = (int)(e / p.per_group);
-  auto state_of = [&](int s) { return s / 4 * 4 * L + l * 4 + s % 4; };
 
-  float h[kRows][S], x[kRows], step[kRows];
+  // a quad of the lane: states 4 L k + 4 l on; there: how many of them exist
+  auto quad = [&](int k) { return k * 4 * L + l * 4; };
+  float4 h[kRows][Q];
+  Raw vb[kRows][Q], vc[kRows][Q];
+  T x[kRows], dt[kRows], z[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t b = min(b0 + r, p.B - 1);
     const bool fresh = p.state_in == nullptr || (p.pos != nullptr && pos_is_zero(p.pos, p.pos64, b));
     const float* from = p.state_in + (b * p.E + e) * p.N;
+    const T* rb = static_cast<const T*>(p.b) + b * p.b_batch + (int64_t)g * p.N;
+    const T* rc = static_cast<const T*>(p.c) + b * p.c_batch + (int64_t)g * p.N;
 #pragma unroll
-    for (int s = 0; s < S; s += 4) {
-      const int n = state_of(s);
+    for (int k = 0; k < Q; ++k) {
+      const int n = quad(k);
+      h[r][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      vb[r][k] = vc[r][k] = Raw{};
       if (kVec) {
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (!fresh && n < p.N) v = *reinterpret_cast<const float4*>(from + n);
-        h[r][s] = v.x; h[r][s + 1] = v.y; h[r][s + 2] = v.z; h[r][s + 3] = v.w;
+        if (n < p.N) {
+          if (!fresh) h[r][k] = *reinterpret_cast<const float4*>(from + n);
+          vb[r][k] = *reinterpret_cast<const Raw*>(rb + n);
+          vc[r][k] = *reinterpret_cast<const Raw*>(rc + n);
+        }
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[r][s + i] = !fresh && n + i < p.N ? from[n + i] : 0.0f;
+        for (int i = 0; i < 4; ++i) {
+          if (n + i < p.N) {
+            if (!fresh) (&h[r][k].x)[i] = from[n + i];
+            reinterpret_cast<T*>(&vb[r][k])[i] = rb[n + i];
+            reinterpret_cast<T*>(&vc[r][k])[i] = rc[n + i];
+          }
+        }
       }
     }
-    x[r] = static_cast<float>(static_cast<const T*>(p.x)[b * p.x_batch + e]);
-    step[r] = static_cast<float>(static_cast<const T*>(p.dt)[b * p.dt_batch + e]);
+    x[r] = static_cast<const T*>(p.x)[b * p.x_batch + e];
+    dt[r] = static_cast<const T*>(p.dt)[b * p.dt_batch + e];
+    z[r] = p.z != nullptr ? static_cast<const T*>(p.z)[b * p.z_batch + e] : T(0.0f);
   }
   float a2[S];
 #pragma unroll
-  for (int s = 0; s < S; ++s) a2[s] = state_of(s) < p.N ? p.a[e * p.N + state_of(s)] * kLog2e : 0.0f;
+  for (int k = 0; k < Q; ++k) {
+    const int n = quad(k);
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (kVec && p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.a) % 16 == 0) {
+      if (n < p.N) v = *reinterpret_cast<const float4*>(p.a + e * p.N + n);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (n + i < p.N) (&v.x)[i] = p.a[e * p.N + n + i];
+      }
+    }
+    a2[4 * k] = v.x * kLog2e; a2[4 * k + 1] = v.y * kLog2e; a2[4 * k + 2] = v.z * kLog2e; a2[4 * k + 3] = v.w * kLog2e;
+  }
   const float bias = p.dt_bias != nullptr ? p.dt_bias[e] : 0.0f, d = p.d != nullptr ? p.d[e] : 0.0f;
 
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t b = b0 + r;
     if (b >= p.B) break;
-    const T* vb = static_cast<const T*>(p.b) + b * p.b_batch + (int64_t)g * p.N;
-    const T* vc = static_cast<const T*>(p.c) + b * p.c_batch + (int64_t)g * p.N;
-    float now = step[r] + bias;
+    const float xr = static_cast<float>(x[r]);
+    float now = static_cast<float>(dt[r]) + bias;
     if (p.softplus) now = softplus_steps(now, now).x;
-    const float put = now * x[r];
+    const float put = now * xr;
     float sum = 0.0f;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int n = state_of(s);
-      if (n < p.N) {
-        h[r][s] = fmaf(exp2_fast(now * a2[s]), h[r][s], put * static_cast<float>(vb[n]));
-        sum = fmaf(h[r][s], static_cast<float>(vc[n]), sum);
-      }
-    }
-    if (p.state_out != nullptr && in) {
-      float* to = p.state_out + (b * p.E + e) * p.N;
+    for (int k = 0; k < Q; ++k) {
+      const int n = quad(k);
+      float fb[4], fc[4], fh[4];
+      widen4(vb[r][k], fb);
+      widen4(vc[r][k], fc);
+      widen4(h[r][k], fh);
 #pragma unroll
-      for (int s = 0; s < S; s += 4) {
-        const int n = state_of(s);
+      for (int i = 0; i < 4; ++i) {
+        fh[i] = fmaf(exp2_fast(now * a2[4 * k + i]), fh[i], put * fb[i]);
+        sum = fmaf(fh[i], fc[i], sum);
+      }
+      if (p.state_out != nullptr && in) {
+        float* to = p.state_out + (b * p.E + e) * p.N + n;
         if (kVec) {
-          if (n < p.N) *reinterpret_cast<float4*>(to + n) = make_float4(h[r][s], h[r][s + 1], h[r][s + 2], h[r][s + 3]);
+          if (n < p.N) *reinterpret_cast<float4*>(to) = make_float4(fh[0], fh[1], fh[2], fh[3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (n + i < p.N) to[n + i] = h[r][s + i];
+            if (n + i < p.N) to[i] = fh[i];
           }
         }
       }
@@ -600,11 +639,8 @@ selective_step_kernel(const SelectiveArgs p) {
 #pragma unroll
     for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (l == 0 && in) {
-      float out = fmaf(d, x[r], sum);
-      if (p.z != nullptr) {
-        const float z = static_cast<float>(static_cast<const T*>(p.z)[b * p.z_batch + e]);
-        out *= silu_fast(z, z).x;
-      }
+      float out = fmaf(d, xr, sum);
+      if (p.z != nullptr) out *= silu_fast(static_cast<float>(z[r]), 0.0f).x;
       static_cast<T*>(p.y)[b * p.E + e] = static_cast<T>(out);
     }
   }
@@ -612,8 +648,11 @@ selective_step_kernel(const SelectiveArgs p) {
 
 template <typename T, int S, int L>
 cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
-  const bool vec = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.state_in) % 16 == 0 &&
-                   reinterpret_cast<uintptr_t>(p.state_out) % 16 == 0;
+  auto fits = [&](const void* q, int64_t batch, int size) {
+    return (reinterpret_cast<uintptr_t>(q) | (uint64_t)(batch * size)) % (4 * size) == 0;
+  };
+  const bool vec = p.N % 4 == 0 && fits(p.state_in, 0, 4) && fits(p.state_out, 0, 4) && fits(p.b, p.b_batch, sizeof(T)) &&
+                   fits(p.c, p.c_batch, sizeof(T));
   const unsigned across = (unsigned)((p.E + 256 / L - 1) / (256 / L));
   // four sequences a thread where they still give every SM its threads
   const bool many = across * p.B >= 4 * 8 * 148;
