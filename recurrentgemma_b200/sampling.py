@@ -2,21 +2,28 @@
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Union
+import math
+from typing import Dict, Optional, Union
 
 import torch
 
 from recurrentgemma_b200 import _lib
 
 
-def _per_row(name: str, value, dtype: torch.dtype, logits: torch.Tensor) -> Optional[torch.Tensor]:
-  """A setting given for each row as a dense tensor; None if it is one number for all."""
-  if not torch.is_tensor(value):
-    return None
-  if value.dtype != dtype:
-    raise TypeError(f"{name} is {value.dtype}: one value for each row is {dtype}")
-  assert value.shape == logits.shape[:-1], (name, value.shape, logits.shape)
-  return value.contiguous()
+def check_settings(temperature, top_k, top_p, min_p, shape) -> Dict[str, Union[float, int, torch.Tensor]]:
+  """The settings by name, if each is a number in its range or a tensor of the given shape and its type."""
+  settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+  for name, value in settings.items():
+    if torch.is_tensor(value):
+      dtype = torch.int32 if name == "top_k" else torch.float32
+      if value.dtype != dtype:
+        raise TypeError(f"{name} is {value.dtype}: one value for each row is {dtype}")
+      assert value.shape == shape, (name, value.shape, shape)
+    elif name == "top_k":
+      settings[name] = max(-1, min(int(value), 2**31 - 1))
+    elif not 0.0 <= value <= (1.0 if name == "min_p" else math.inf):
+      raise ValueError(f"{name} {value}: a temperature and top_p are at least 0, min_p is from 0 to 1")
+  return settings
 
 
 def sample(
@@ -45,25 +52,21 @@ def sample(
 
 @torch.no_grad()
 def _sample(logits, uniforms, temperature, top_k, top_p, min_p, out):
-  settings = (temperature, top_k, top_p, min_p)
-  dev = _lib.require_cuda(logits, uniforms, *(s for s in settings if torch.is_tensor(s)), out)
+  settings = check_settings(temperature, top_k, top_p, min_p, logits.shape[:-1])
+  dev = _lib.require_cuda(logits, uniforms, *(s for s in settings.values() if torch.is_tensor(s)), out)
   v = logits.shape[-1]
   if uniforms.dtype != torch.float32:
     raise TypeError(f"uniforms are {uniforms.dtype}, not float32")
   assert uniforms.shape == logits.shape[:-1], (uniforms.shape, logits.shape)
-  rows = [_per_row(name, value, torch.int32 if name == "top_k" else torch.float32, logits)
-          for name, value in zip(("temperature", "top_k", "top_p", "min_p"), settings)]
-  numbers = [value if row is None else 0 for value, row in zip(settings, rows)]
-  if not numbers[0] >= 0 or not numbers[2] >= 0 or not 0 <= numbers[3] <= 1:
-    raise ValueError(f"temperature {numbers[0]}, top_p {numbers[2]}, min_p {numbers[3]}: a temperature and top_p "
-                     "of at least 0, min_p from 0 to 1")
+  rows = {n: s.contiguous() if torch.is_tensor(s) else None for n, s in settings.items()}
+  numbers = {n: 0 if torch.is_tensor(s) else s for n, s in settings.items()}
   x = logits if logits.ndim == 2 and logits.stride(1) == 1 else logits.contiguous()
   uc = uniforms.contiguous()
   if out is None:
     out = torch.empty(logits.shape[:-1], dtype=torch.int32, device=dev)
   assert out.shape == logits.shape[:-1] and out.dtype == torch.int32 and out.is_contiguous()
-  p = _lib.RgkSampleSettings(*(_lib.ptr(r) for r in rows), float(numbers[0]), min(int(numbers[1]), 2**31 - 1),
-                             float(numbers[2]), float(numbers[3]))
+  p = _lib.RgkSampleSettings(**{n: _lib.ptr(r) for n, r in rows.items()},
+                             **{f"{n}_value": value for n, value in numbers.items()})
   with torch.cuda.device(dev):
     _lib.check(_lib.load().rgk_sample(
         x.data_ptr(), uc.numel(), v, x.stride(0) if x.ndim == 2 else v, _lib.dtype_code(logits.dtype),
