@@ -510,7 +510,8 @@ cudaError_t launch_kernel(SelectiveArgs p, cudaStream_t s) {
     const int64_t most = min((int64_t)per_sm, p.blocks / sms);
     if (most > 0 && most * sms < p.blocks && p.blocks <= kMostBlocks) {
       grid = most * sms;
-      p.chunk = max((int64_t)128, (p.T / 24 + Sh::kTile - 1) / Sh::kTile * Sh::kTile);
+      // (24 of them: the last round is short of 4 % at most; no longer than a wait for one is given)
+      p.chunk = min((int64_t)4096, max((int64_t)128, (p.T / 24 + Sh::kTile - 1) / Sh::kTile * Sh::kTile));
       p.chunks = (p.T + p.chunk - 1) / p.chunk;
       p.done = reinterpret_cast<int*>(p.header + 1);
       if ((e = cudaMemsetAsync(&p.header->ticket, 0, sizeof(WsHeader) - sizeof(int) + p.blocks * sizeof(int), s)) != cudaSuccess)
