@@ -15,7 +15,8 @@
 // that it ends in hold at most 2048 tokens, those are brought together in index order, and one CTA sorts them and does
 // the rest; otherwise the bin's own tokens are, which gives the last token kept, and the draw runs over the row.  A bin
 // with more tokens than that (ties, huge temperatures) is cut into 2048 ranges of keys, and again if need be; a single
-// key is cut by counting.
+// key is cut by counting.  For top-k up to 128 there is no histogram: the k-th largest of the maxima of 128 parts of the
+// row bounds what can be among the first k.
 //
 // Bound: 2 or 4 bytes a token from HBM, and for whole rows and top-p without top-k the 64-bit exponential of every token
 // within 31 temperatures of the maximum (11 double-precision operations, 2 cycles of a scheduler each).
@@ -41,6 +42,7 @@ constexpr int kMostParts = 8;
 constexpr float kRange = 32.0f;                                   // temperatures below the maximum: W = 0 from 31.2 on
 constexpr int kTable = 64;
 constexpr int kStretches = 16;
+constexpr int kGroups = 128;                                      // of a row's threads
 
 // The order of the floats as an order of integers (-0 counts as 0, NaN below everything).
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -140,6 +142,7 @@ struct Shared {
   float best[kMostParts];
   int best_at[kMostParts];
   unsigned key_lo[kMostParts], key_hi[kMostParts];
+  float groups[kGroups], least;                                   // maxima of parts of the row, and one of them
   Found found;
   unsigned length;                                                // of the list
   unsigned mine, place;                                           // of it in this CTA: how many, and from where on
@@ -413,7 +416,8 @@ __device__ Found histogram(const Row<T>& row, Shared& sh, const Binning& bins, c
 }
 
 // Brings the tokens that `wanted` picks, 2048 at most, together in the first CTA, in any order, as sort_list's words:
-// in each CTA first (in `kept`), then with one place for all of a CTA's in the first one's `order`.
+// in each CTA first (in `kept`), then with one place for all of a CTA's in the first one's `order`.  How many there are,
+// which may be more than the list holds: then it is of no use.
 template <typename T, typename F>
 __device__ int gather(const Row<T>& row, Shared& sh, F&& wanted) {
   if (threadIdx.x == 0) sh.mine = sh.length = 0;
@@ -434,13 +438,15 @@ __device__ int gather(const Row<T>& row, Shared& sh, F&& wanted) {
   __syncthreads();
   const unsigned n = min(sh.mine, (unsigned)kList);
   Shared* first = row.parts > 1 ? peer(&sh, 0) : &sh;
-  if (threadIdx.x == 0) sh.place = atomicAdd(&first->length, n);
+  if (threadIdx.x == 0) sh.place = atomicAdd(&first->length, sh.mine);
   __syncthreads();
   for (unsigned i = threadIdx.x; i < n; i += kThreads) {
     if (sh.place + i < kList) first->order[sh.place + i] = sh.kept[i];
   }
   row.sync();
-  return min(sh.length, (unsigned)kList);                         // (of use in the first CTA)
+  const int all = (int)first->length;
+  row.sync();
+  return all;
 }
 
 // Sorts the first n words of `words`, which are all different, ascending: short lists by counting what is smaller, long
@@ -650,8 +656,13 @@ sample_kernel(const SampleArgs p, int parts) {
   auto better = [&](float ob, int oa) {
     if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
   };
+  const int group = kThreads * parts / kGroups;                   // lanes: 4, 8, 16 or 32
+  float of_group = best;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
+  for (int o = 1; o < 32; o <<= 1) {
+    better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
+    if (2 * o == group) of_group = best;
+  }
   if (lane == 0) {
     sh.part[warp] = (u64)__float_as_uint(best) << 32 | (unsigned)at;
   }
@@ -661,6 +672,9 @@ sample_kernel(const SampleArgs p, int parts) {
   if (tid < parts) {
     peer(&sh, tid)->best[row.rank] = best;
     peer(&sh, tid)->best_at[row.rank] = at;
+  }
+  if (lane % group == 0) {
+    for (int r = 0; r < parts; ++r) peer(&sh, r)->groups[(row.rank * kThreads + tid) / group] = of_group;
   }
   row.sync();
   for (int r = 0; r < parts; ++r) better(sh.best[r], sh.best_at[r]);
@@ -696,7 +710,22 @@ sample_kernel(const SampleArgs p, int parts) {
   int n = 0;
   u64 wanted = 0;
   bool listed = false;
-  if (set.top_k > 0) listed = prefix<true, false>(row, sh, weight, bins, best, cut, -1.0, (u64)set.top_k, &cut, &n, &wanted);
+  if (set.top_k > 0 && set.top_k <= kGroups) {
+    // The k-th largest of the groups' maxima: k tokens are at least that, so the first k of all are among those that
+    // are.  Mostly they are few (some 60 for k = 50, 600 for k = 128).
+    if (tid < kGroups) {
+      const float mine = sh.groups[tid];
+      int place = 0;
+#pragma unroll 8
+      for (int i = 0; i < kGroups; ++i) place += sh.groups[i] > mine || (sh.groups[i] == mine && i < tid);
+      if (place == set.top_k - 1) sh.least = mine;
+    }
+    __syncthreads();
+    const float least = sh.least;
+    n = gather(row, sh, [&](float l, int) { return l >= least && l > cut.end; });
+    listed = n <= kList;
+  }
+  if (!listed && set.top_k > 0) listed = prefix<true, false>(row, sh, weight, bins, best, cut, -1.0, (u64)set.top_k, &cut, &n, &wanted);
   if (!listed && set.top_p < 1.0f) {
     set.top_k = 0;                                                // (in the cut by now)
     const double share = fmax((double)set.top_p, 0.0);

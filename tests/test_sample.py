@@ -50,7 +50,7 @@ def rows(seed, m, v, dtype, std=3.0):
 
 SETTINGS = [
     {}, dict(temperature=0.0), dict(temperature=0.05), dict(temperature=40.0), dict(top_k=1), dict(top_k=2),
-    dict(top_k=40), dict(top_k=10**6), dict(top_p=0.0), dict(top_p=0.5), dict(top_p=0.95), dict(top_p=0.9999),
+    dict(top_k=40), dict(top_k=128), dict(top_k=129), dict(top_k=3000, top_p=0.9), dict(top_k=10**6), dict(top_p=0.0), dict(top_p=0.5), dict(top_p=0.95), dict(top_p=0.9999),
     dict(min_p=0.1), dict(min_p=1.0), dict(top_k=100, top_p=0.7, min_p=0.02, temperature=1.3),
     dict(top_p=0.9, temperature=6.0),
 ]
@@ -96,7 +96,7 @@ def test_sample_special_rows(dtype):
   import recurrentgemma_b200 as rg
   v = 5000
   low = torch.finfo(dtype).min
-  logits, uniforms, _ = rows(1, 15, v, dtype)
+  logits, uniforms, _ = rows(1, 17, v, dtype)
   logits[0] = 0.0
   logits[1] = -math.inf
   logits[2] = math.nan
@@ -115,6 +115,8 @@ def test_sample_special_rows(dtype):
   logits[13, 1:] = -math.inf
   logits[14] = -math.inf
   logits[14, v - 1] = low
+  logits[15, 1000:1300] += 20.0                       # the likely ones side by side
+  logits[16, :40], logits[16, 2500:2600] = 9.0, 9.0   # and equal
   for settings in SETTINGS:
     for u in (0.0, 0.3, 0.5, 1.0 - 2.0 ** -24):
       uniforms[:] = u
