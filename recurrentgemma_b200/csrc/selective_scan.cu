@@ -36,15 +36,18 @@ constexpr unsigned kWaitLimit = 1u << 23;                       // polls, 0.2 us
 // softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1]: log1p(e) / e by a polynomial fitted for the
 // smallest largest relative error on [0, 1] (5e-9; 1.8e-7 in float32 arithmetic).  Steps of 1e-3 come out with their
 // relative precision, which the hardware logarithm of 1 + e would lose.  (A NaN stays one: e is.)
-__device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
-  const float2 arg = split(mul2(pair(fabsf(v0), fabsf(v1)), pair(-kLog2e, -kLog2e)));
-  const Pair e = pair(exp2_fast(arg.x), exp2_fast(arg.y));
+constexpr float softplus_coefficient(int i) {
   constexpr float k[10] = {1.0f, -0.4999990165233612f, 0.3332996368408203f, -0.24954134225845337f,
                            0.1967593878507614f, -0.15305590629577637f, 0.10603651404380798f,
                            -0.056959498673677444f, 0.01985144428908825f, -0.0032440212089568377f};
-  Pair p = pair(k[9], k[9]);
+  return k[i];
+}
+__device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
+  const float2 arg = split(mul2(pair(fabsf(v0), fabsf(v1)), pair(-kLog2e, -kLog2e)));
+  const Pair e = pair(exp2_fast(arg.x), exp2_fast(arg.y));
+  Pair p = pair(softplus_coefficient(9), softplus_coefficient(9));
 #pragma unroll
-  for (int i = 8; i >= 0; --i) p = fma2(p, e, pair(k[i], k[i]));
+  for (int i = 8; i >= 0; --i) p = fma2(p, e, pair(softplus_coefficient(i), softplus_coefficient(i)));
   return split(fma2(p, e, pair(fmaxf(v0, 0.0f), fmaxf(v1, 0.0f))));
 }
 
@@ -534,6 +537,14 @@ cudaError_t launch(const SelectiveArgs& p, cudaStream_t s) {
 // of kRows sequences, L lanes a channel, so that a, d and the bias are read once for kRows sequences and all that is
 // read of kRows sequences is in flight at a time.  kVec: states, b and c are read and written four at a time.  256 x 5120
 // x 16 in bfloat16: 48 us.
+__device__ __forceinline__ float softplus_step(float v) {        // softplus_steps for one
+  const float e = exp2_fast(-fabsf(v) * kLog2e);
+  float q = softplus_coefficient(9);
+#pragma unroll
+  for (int i = 8; i >= 0; --i) q = fmaf(q, e, softplus_coefficient(i));
+  return fmaf(q, e, fmaxf(v, 0.0f));
+}
+
 template <typename T> struct Four;                               // four elements as they lie in memory
 template <> struct Four<float> { using type = float4; };
 template <> struct Four<__nv_bfloat16> { using type = uint2; };
@@ -652,6 +663,101 @@ selective_step_kernel(const SelectiveArgs p) {
   }
 }
 
+// The same for many sequences: a thread goes through kDepth and more of them with the same four states of a channel, whose
+// values come by copies that run kDepth sequences ahead into places of its own in shared memory (nobody else reads them:
+// no barriers), the rest of a sequence a step ahead into registers.  256 x 5120 x 16 in bfloat16: 48 us with
+// four sequences a thread, 43 so (64 % of the measured copy rate).
+// (Addresses run along: products of 64 bits for every row were most of its 237 instructions, which bound it.)
+template <typename T, int L>
+__global__ void __launch_bounds__(256, 4)
+selective_steps_kernel(const SelectiveArgs p, int per) {
+  using Raw = typename Four<T>::type;
+  constexpr int kDepth = 8;
+  __shared__ float4 ring[kDepth][256];
+  const int64_t at = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const int l = threadIdx.x % L;
+  const bool in = at < p.E;
+  const int64_t e = in ? at : p.E - 1;                           // (whole groups of lanes: they shuffle)
+  const bool there = l * 4 < p.N, mine = in && there;
+  const int n = there ? l * 4 : 0;                               // (a lane too many reads what the first one does)
+  const int64_t b0 = (int64_t)blockIdx.y * per;
+  const int rows = (int)min((int64_t)per, p.B - b0), g = (int)(e / p.per_group);
+
+  const int64_t row = p.E * p.N, place = b0 * row + e * p.N + n; // of a state
+  const bool held = p.state_in != nullptr, gated = p.z != nullptr;
+  const float* from = held ? p.state_in + place : nullptr;
+  float* to = mine && p.state_out != nullptr ? p.state_out + place : nullptr;
+  const T *px = static_cast<const T*>(p.x) + b0 * p.x_batch + e, *pdt = static_cast<const T*>(p.dt) + b0 * p.dt_batch + e;
+  const T* pz = gated ? static_cast<const T*>(p.z) + b0 * p.z_batch + e : px;
+  const int64_t z_batch = gated ? p.z_batch : p.x_batch;
+  const T* pb = static_cast<const T*>(p.b) + b0 * p.b_batch + (int64_t)g * p.N + n;
+  const T* pc = static_cast<const T*>(p.c) + b0 * p.c_batch + (int64_t)g * p.N + n;
+  T* y = static_cast<T*>(p.y) + b0 * p.E + e;
+
+  int asked = 0;
+  auto ask = [&]() {
+    if (held && asked < rows) {
+      copy_async<16>(&ring[asked % kDepth][threadIdx.x], from, true);
+      from += row;
+    }
+    ++asked;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  struct Inputs { Raw b, c; T x, dt, z; };
+  auto inputs = [&]() {
+    Inputs v;
+    v.b = *reinterpret_cast<const Raw*>(pb);
+    v.c = *reinterpret_cast<const Raw*>(pc);
+    v.x = *px; v.dt = *pdt; v.z = *pz;
+    pb += p.b_batch; pc += p.c_batch; px += p.x_batch; pdt += p.dt_batch; pz += z_batch;
+    return v;
+  };
+  for (int r = 0; r < kDepth - 1; ++r) ask();
+  Inputs next = inputs();
+  float a2[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a2[i] = there ? p.a[e * p.N + n + i] * kLog2e : 0.0f;
+  const float bias = p.dt_bias != nullptr ? p.dt_bias[e] : 0.0f, d = p.d != nullptr ? p.d[e] : 0.0f;
+
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r) {
+    ask();                                                       // (where the sequence before this one has been)
+    const Inputs v = next;
+    if (r + 1 < rows) next = inputs();
+    asm volatile("cp.async.wait_group %0;" :: "n"(kDepth - 1) : "memory");
+    float h[4] = {0.0f, 0.0f, 0.0f, 0.0f}, fb[4], fc[4];
+    if (held && !(p.pos != nullptr && pos_is_zero(p.pos, p.pos64, b0 + r))) {
+      const float4 was = ring[r % kDepth][threadIdx.x];
+      h[0] = was.x; h[1] = was.y; h[2] = was.z; h[3] = was.w;
+    }
+    widen4(v.b, fb);
+    widen4(v.c, fc);
+    const float x = static_cast<float>(v.x);
+    float now = static_cast<float>(v.dt) + bias;
+    if (p.softplus) now = softplus_step(now);
+    const float put = now * x;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = fmaf(exp2_fast(now * a2[i]), h[i], put * fb[i]);
+      sum = fmaf(h[i], fc[i], sum);
+    }
+    if (to != nullptr) {
+      *reinterpret_cast<float4*>(to) = make_float4(h[0], h[1], h[2], h[3]);
+      to += row;
+    }
+    sum = there ? sum : 0.0f;
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (l == 0 && in) {
+      float out = fmaf(d, x, sum);
+      if (gated) out *= silu_fast(static_cast<float>(v.z), 0.0f).x;
+      *y = static_cast<T>(out);
+    }
+    y += p.E;
+  }
+}
+
 template <typename T, int S, int L>
 cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
   auto fits = [&](const void* q, int64_t batch, int size) {
@@ -660,6 +766,18 @@ cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
   const bool vec = p.N % 4 == 0 && fits(p.state_in, 0, 4) && fits(p.state_out, 0, 4) && fits(p.b, p.b_batch, sizeof(T)) &&
                    fits(p.c, p.c_batch, sizeof(T));
   const unsigned across = (unsigned)((p.E + 256 / L - 1) / (256 / L));
+  if constexpr (S == 4) {
+    static PerDeviceOnce once;
+    int sms = 0;
+    const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
+    if (e != cudaSuccess) return e;
+    // eight sequences a thread and more where four CTAs an SM have that many
+    const int64_t down = max((int64_t)1, (int64_t)4 * sms / across), per = (p.B + down - 1) / down;
+    if (vec && per >= 8) {
+      selective_steps_kernel<T, L><<<dim3(across, (unsigned)((p.B + per - 1) / per)), 256, 0, s>>>(p, (int)per);
+      return cudaGetLastError();
+    }
+  }
   // four sequences a thread where they still give every SM its threads
   const bool many = across * p.B >= 4 * 8 * 148;
   const dim3 grid(across, (unsigned)(many ? (p.B + 3) / 4 : p.B));

@@ -180,6 +180,8 @@ SCAN = [
     (70, 1, 2560, 16, 1, 0, {}),
     (67, 1, 2570, 9, 2, 3, dict(part=True)),
     (131, 1, 300, 130, 1, 0, dict(z=False)),
+    (256, 1, 5120, 16, 1, 2, {}),                  # many sequences a thread
+    (300, 1, 5132, 8, 2, 0, dict(state=False)),
     (1, 2, 8, 1, 1, 0, {}),
     (2, 31, 64, 16, 2, 7, {}),
     (2, 32, 36, 16, 1, 0, dict(state=False)),
