@@ -204,6 +204,30 @@ selective_scan_kernel(const SelectiveArgs p) {
       const T *qx = x + (begin + xr) * p.x_token + xc, *qd = dt + (begin + xr) * p.dt_token + xc;
       const T* qz = z == nullptr ? nullptr : z + (begin + xr) * p.z_token + xc;
       const T *qb = bb + (begin + nr) * p.b_token + nc, *qc = cc + (begin + nr) * p.c_token + nc;
+      // b and c of two-byte elements whose rows begin anywhere: no copy takes them, so they come through registers, loaded
+      // when the tile is asked for and stored when it is wanted
+      constexpr bool kStaged = !kAligned && sizeof(T) == 2;
+      constexpr int kHeld = kStaged ? (kTile * kPad + kTeam - 1) / kTeam : 1;
+      T on_way[2][kHeld];
+      auto load_rows = [&](const T* src, int64_t stride, int rows, T (&to)[kHeld]) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+          const int i = tid + k * kTeam, r = i / kPad, n = i % kPad;
+          to[k] = r < rows && n < p.N ? src[r * stride + n] : T(0.0f);
+        }
+      };
+      auto settle = [&](int tile) {
+        if (kStaged && p.copy_n < 4) {
+#pragma unroll
+          for (int k = 0; k < kHeld; ++k) {
+            const int i = tid + k * kTeam;
+            if (kTile * kPad % kTeam == 0 || i < kTile * kPad) {
+              raw_n(tile % 3, 0)[i] = on_way[0][k];
+              raw_n(tile % 3, 1)[i] = on_way[1][k];
+            }
+          }
+        }
+      };
       auto ask = [&](int tile) {
         const int64_t t0 = begin + (int64_t)tile * kTile;
         const int stage = tile % 3, rows = (int)min((int64_t)kTile, end - t0);
@@ -231,8 +255,13 @@ selective_scan_kernel(const SelectiveArgs p) {
           fetch_rows<T, kAligned, kTeam, kTile, kChan>(tid, p.copy_x, raw(stage, 1), dt + t0 * p.dt_token, p.dt_token, rows, kChan, there);
           if (z != nullptr)
             fetch_rows<T, kAligned, kTeam, kTile, kChan>(tid, p.copy_x, raw(stage, 2), z + t0 * p.z_token, p.z_token, rows, kChan, there);
-          fetch_rows<T, kAligned, kTeam, kTile, kPad>(tid, p.copy_n, raw_n(stage, 0), bb + t0 * p.b_token, p.b_token, rows, p.N, p.N);
-          fetch_rows<T, kAligned, kTeam, kTile, kPad>(tid, p.copy_n, raw_n(stage, 1), cc + t0 * p.c_token, p.c_token, rows, p.N, p.N);
+          if (kStaged && p.copy_n < 4) {
+            load_rows(bb + t0 * p.b_token, p.b_token, rows, on_way[0]);
+            load_rows(cc + t0 * p.c_token, p.c_token, rows, on_way[1]);
+          } else {
+            fetch_rows<T, kAligned, kTeam, kTile, kPad>(tid, p.copy_n, raw_n(stage, 0), bb + t0 * p.b_token, p.b_token, rows, p.N, p.N);
+            fetch_rows<T, kAligned, kTeam, kTile, kPad>(tid, p.copy_n, raw_n(stage, 1), cc + t0 * p.c_token, p.c_token, rows, p.N, p.N);
+          }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
@@ -360,6 +389,7 @@ selective_scan_kernel(const SelectiveArgs p) {
       bool start = starts_at(0);
 #pragma unroll 1
       for (int tile = 0; tile < tiles; ++tile) {
+        settle(tile);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         meet<kTeam>(kHelpersMeet);                               // the tile is here, tile - 2 is done with
         if (tile + 1 < tiles) ask(tile + 1);
