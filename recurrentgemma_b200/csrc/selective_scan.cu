@@ -828,40 +828,64 @@ cudaError_t launch_step_states(const SelectiveArgs& p, cudaStream_t s) {
   return launch_step<T, 8, 32>(p, s);
 }
 
-// What a shape takes, relative: `alone` is its time where every CTA has an SM (us for 2048 steps of 16 states), the
-// factor what blocks behind the first round of SMs add; a second CTA on an SM costs half as much as the first.
-double estimate(double alone, int64_t blocks, int sms) {
-  const double rounds = (double)blocks / sms;
-  return alone * (rounds <= 1.0 ? 1.0 : rounds < 2.0 ? rounds + 0.45 : rounds);
+// There is a choice of shapes: few states a thread keep a step short where channels are few, many states and two channels
+// share what is read from shared memory where they are many.  What a shape takes, relative: `alone` is its time where every CTA
+// has an SM (us for 1024 steps), the factor what blocks behind the first round of SMs add; a second CTA on an SM costs
+// half as much as the first.
+struct Choice { double alone; int channels; };                   // channels of a CTA
+template <int kCount>
+int quickest(const Choice (&of)[kCount], const SelectiveArgs& p, int sms) {
+  int best = 0;
+  double least = 0.0;
+  for (int i = 0; i < kCount; ++i) {
+    const int64_t blocks = (p.per_group + of[i].channels - 1) / of[i].channels * p.groups * p.B;
+    const double rounds = (double)blocks / sms;
+    const double time = of[i].alone * (rounds <= 1.0 ? 1.0 : rounds < 2.0 ? rounds + 0.45 : rounds);
+    if (i == 0 || time < least) { best = i; least = time; }
+  }
+  return best;
 }
 
-// Up to 16 states there is a choice: few states a thread keep a step short where channels are few, many states and
-// two channels share what is read from shared memory where they are many.  Measured in bfloat16, 2048 steps of 1280 /
-// 4096 / 5120 / 10240 / 15360 / 20480 channels: 2 states 70 / 183 / 154 / 292 / 430 / 569 us, 4 states 89 / 89 / 146 /
-// 193 / 282 / 372, 8 states 134 / 134 / 134 / 202 / 295 / 293, 8 of two channels 243 / 242 / 242 / 240 / 240 / 348;
-// 4096 steps of 40960 channels: 2026 / 1325 / 1039 / 988.
+// Measured in bfloat16, 1024 steps of 2560 / 10240 / 20480 / 40960 channels (16 states: 2048 steps of 4096 / 10240 / 20480),
+// in the order of the shapes:   8 states 57 / 85 / 113 / 214, 96 / 95 / 133 / 184;   16 states 183 / 292 / 569, 89 / 193 /
+// 372, 134 / 202 / 293, 242 / 240 / 348;   32 states 74 / 194 / 378 / 743, 69 / 142 / 271 / 529, 112 / 155 / 238 / 444;
+// 64 states 120 / 443 / 875 / 1734, 104 / 285 / 554 / 1091, 114 / 236 / 440 / 870;   128 states 168 / 627 / 1237,
+// 191 / 497 / 989.
 template <typename T>
 cudaError_t launch_states(const SelectiveArgs& p, cudaStream_t s) {
+  static PerDeviceOnce once;
+  int sms = 0;
+  const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
+  if (e != cudaSuccess) return e;
   if (p.N <= 4) return launch<T, 4, 1, 1, 16>(p, s);
-  if (p.N <= 8) return launch<T, 4, 1, 2, 16>(p, s);
-  if (p.N <= 16) {
-    static PerDeviceOnce once;
-    int sms = 0;
-    const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
-    if (e != cudaSuccess) return e;
-    auto blocks = [&](int channels) { return (p.per_group + channels - 1) / channels * p.groups * p.B; };
-    const double by[4] = {estimate(70, blocks(16), sms), estimate(89, blocks(32), sms), estimate(134, blocks(64), sms),
-                          estimate(242, blocks(128), sms)};
-    int best = 0;
-    for (int i = 1; i < 4; ++i) best = by[i] < by[best] ? i : best;
-    return best == 0   ? launch<T, 2, 1, 8, 32>(p, s)
-           : best == 1 ? launch<T, 4, 1, 4, 32>(p, s)
-           : best == 2 ? launch<T, 8, 1, 2, 16>(p, s)
-                       : launch<T, 8, 2, 2, 16>(p, s);
+  if (p.N <= 8) {
+    return quickest({{57, 64}, {95, 128}}, p, sms) == 0 ? launch<T, 4, 1, 2, 16>(p, s) : launch<T, 4, 2, 2, 16>(p, s);
   }
-  if (p.N <= 32) return launch<T, 4, 1, 8, 32>(p, s);
-  if (p.N <= 64) return launch<T, 4, 1, 16, 16>(p, s);
-  if (p.N <= 128) return launch<T, 4, 1, 32, 16>(p, s);
+  if (p.N <= 16) {
+    switch (quickest({{35, 16}, {44.5, 32}, {67, 64}, {121, 128}}, p, sms)) {
+      case 0: return launch<T, 2, 1, 8, 32>(p, s);
+      case 1: return launch<T, 4, 1, 4, 32>(p, s);
+      case 2: return launch<T, 8, 1, 2, 16>(p, s);
+      default: return launch<T, 8, 2, 2, 16>(p, s);
+    }
+  }
+  if (p.N <= 32) {
+    switch (quickest({{48, 16}, {66, 32}, {112, 64}}, p, sms)) {
+      case 0: return launch<T, 4, 1, 8, 32>(p, s);
+      case 1: return launch<T, 8, 1, 4, 16>(p, s);
+      default: return launch<T, 8, 2, 4, 16>(p, s);
+    }
+  }
+  if (p.N <= 64) {
+    switch (quickest({{65, 8}, {75, 16}, {112, 32}}, p, sms)) {
+      case 0: return launch<T, 4, 1, 16, 16>(p, s);
+      case 1: return launch<T, 8, 1, 8, 16>(p, s);
+      default: return launch<T, 8, 2, 8, 16>(p, s);
+    }
+  }
+  if (p.N <= 128) {
+    return quickest({{86, 8}, {149, 16}}, p, sms) == 0 ? launch<T, 8, 1, 16, 16>(p, s) : launch<T, 8, 2, 16, 8>(p, s);
+  }
   return launch<T, 8, 1, 32, 8>(p, s);
 }
 

@@ -194,6 +194,9 @@ SCAN = [
     (2, 35, 10, 256, 1, 8, dict(part=True)),
     (3, 257, 2560, 16, 1, 60, {}),
     (9, 90, 5120, 16, 1, 0, {}),
+    (1, 50, 1024, 16, 1, 20, {}), (1, 50, 4096, 16, 1, 20, {}),        # every shape that a number of states has
+    (8, 40, 5120, 8, 1, 30, {}), (2, 40, 5120, 30, 2, 30, dict(part=True)), (4, 40, 5120, 32, 1, 0, {}),
+    (2, 40, 2560, 64, 1, 30, {}), (2, 40, 5120, 60, 1, 30, {}), (1, 40, 5120, 128, 2, 30, {}),
     (3, 700, 5120, 16, 1, 90, {}),                 # more blocks of channels than CTAs: chunks of time
     (2, 1031, 5120, 24, 2, 200, dict(part=True)),
 ]
