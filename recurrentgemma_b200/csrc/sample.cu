@@ -541,8 +541,8 @@ __device__ int finish_list(Shared& sh, int n, const Weights& weight, const Setti
 // The shortest prefix of what `was` keeps with `target` tokens, or with `share` of the weight.  True: it, and everything
 // in front of it, is in a list of `*n` tokens, where `*wanted` is to be reached; else *cut is its end.
 template <bool kCount, bool kTies, typename T>
-__device__ bool prefix(const Row<T>& row, Shared& sh, const Weights& weight, Binning bins, float largest, const Cut was, double share,
-                       u64 target, Cut* cut, int* n, u64* wanted) {
+__device__ bool prefix(const Row<T>& row, Shared& sh, const Weights& weight, Binning bins, float largest, const Cut was,
+                       double share, u64 target, Cut* cut, int* n, u64* wanted) {
   *cut = was;
   const Test<kTies> eligible{was};
   Found f = histogram<kCount>(row, sh, bins, weight, eligible, share, target);
@@ -638,7 +638,8 @@ sample_kernel(const SampleArgs p, int parts) {
   row.parts = parts;
   row.rank = (int)(blockIdx.x - m * parts);
   const int packs = (row.head + row.V + kPer - 1) / kPer;
-  const int run = (packs + parts * kWarps - 1) / (parts * kWarps);
+  int run = (packs + parts * kWarps - 1) / (parts * kWarps);
+  if (run > 64) run = (run + 32 * kAhead - 1) / (32 * kAhead) * (32 * kAhead);        // (whole rounds of `each`)
   row.begin = min(packs, (row.rank * kWarps + warp) * run);
   row.end = min(packs, row.begin + run);
   if (parts > 1) cluster_arrive();                                // "this CTA runs"
@@ -725,7 +726,8 @@ sample_kernel(const SampleArgs p, int parts) {
     n = gather(row, sh, [&](float l, int) { return l >= least && l > cut.end; });
     listed = n <= kList;
   }
-  if (!listed && set.top_k > 0) listed = prefix<true, false>(row, sh, weight, bins, best, cut, -1.0, (u64)set.top_k, &cut, &n, &wanted);
+  if (!listed && set.top_k > 0)
+    listed = prefix<true, false>(row, sh, weight, bins, best, cut, -1.0, (u64)set.top_k, &cut, &n, &wanted);
   if (!listed && set.top_p < 1.0f) {
     set.top_k = 0;                                                // (in the cut by now)
     const double share = fmax((double)set.top_p, 0.0);
