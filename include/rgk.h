@@ -493,8 +493,9 @@ RGK_API int rgk_geglu_bias(const void* up, const void* bias, int64_t M, int64_t 
  *     y_t = (sum_n h_t[n] c_t[g,n] + d[e] x_t) silu(z_t).
  *   x, dt, z (or NULL) [B,T,E], b, c [B,T,groups,N]; a [E,N], d [E] or NULL, dt_bias [E] or NULL and the
  *   states [B,E,N] are float32.  state_in NULL: zeros; state_out: NULL, or it may be state_in.  T may be 0.
- *   workspace: NULL, or rgk_selective_scan_workspace_bytes() of scratch, with which long calls of many
- *   channels share out the device more evenly.
+ *   workspace: NULL, or rgk_selective_scan_workspace_bytes() of scratch (4-byte aligned, of any content, of no other
+ *   call at the time), with which long calls of many channels share out the device more evenly.  status: a word
+ *   that a wait which gives up raises to RGK_ETIMEOUT (a workspace's first int), or NULL.
  * rgk_sample: out [M] int32, one token for each row of logits [M,V] (rows row_stride apart; V up to 2^20).
  *   Tokens are ordered by logit, the largest first, equal ones by index.  Kept are the first top_k of them (all for
  *   top_k <= 0), of those, with weights exp((logit - largest) / temperature) rounded to multiples of 2^-44
@@ -519,7 +520,7 @@ typedef struct rgk_scan_inputs {
 RGK_API int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int pos_dtype,
                                const float* state_in, int64_t B, int64_t T, int64_t E, int groups, int N,
                                int dtype, void* y, float* state_out, void* workspace, size_t workspace_bytes,
-                               void* stream);
+                               int* status, void* stream);
 RGK_API size_t rgk_selective_scan_workspace_bytes(void);
 
 typedef struct rgk_sample_settings {

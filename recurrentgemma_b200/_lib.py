@@ -138,7 +138,7 @@ SIGNATURES = {
     "rgk_causal_conv": (_int, [_vp, _i64, _i64, _vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int,
                                _vp, _vp, _vp]),
     "rgk_selective_scan": (_int, [ctypes.POINTER(RgkScanInputs), _vp, _int, _vp, _i64, _i64, _i64, _int, _int,
-                                  _int, _vp, _vp, _vp, _sz, _vp]),
+                                  _int, _vp, _vp, _vp, _sz, _vp, _vp]),
     "rgk_selective_scan_workspace_bytes": (_sz, []),
     "rgk_sample": (_int, [_vp, _i64, _i64, _i64, _int, _vp, ctypes.POINTER(RgkSampleSettings), _vp, _vp]),
     "rgk_add_rmsnorm": (_int, [_vp, _vp, _vp, _i64, _i64, ctypes.c_float, _int, _vp, _vp, _vp]),

@@ -727,7 +727,7 @@ int rgk_causal_conv(const void* x, int64_t x_batch, int64_t x_token, const void*
 
 int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int pos_dtype, const float* state_in,
                        int64_t B, int64_t T, int64_t E, int groups, int N, int dtype, void* y, float* state_out,
-                       void* workspace, size_t workspace_bytes, void* stream) {
+                       void* workspace, size_t workspace_bytes, int* status, void* stream) {
   const int rc = check_sequence(B, T, E, dtype, segment_pos, pos_dtype);
   if (rc != RGK_OK) return rc;
   RGK_REQUIRE(in != nullptr, RGK_EINVAL, "in is NULL");
@@ -743,11 +743,12 @@ int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int p
               "a pointer is not aligned to its elements");
   RGK_REQUIRE(workspace == nullptr || workspace_bytes >= rgk::selective_workspace_bytes(), RGK_EWORKSPACE,
               "workspace of %zu bytes, %zu needed", workspace_bytes, rgk::selective_workspace_bytes());
-  RGK_REQUIRE(aligned_to(workspace, 256), RGK_EALIGN, "the workspace must be 256-byte aligned");
+  RGK_REQUIRE(aligned_to(workspace, 4) && aligned_to(status, 4), RGK_EALIGN, "workspace and status must be 4-byte aligned");
   if (T == 0 && state_out == nullptr) return RGK_OK;
   RGK_CHECK_DEVICE();
   rgk::SelectiveArgs p = {};
-  p.header = static_cast<rgk::WsHeader*>(workspace);
+  p.ticket = static_cast<unsigned*>(workspace);
+  p.status = status;
   p.x = in->x; p.dt = in->dt; p.z = in->z; p.b = in->b; p.c = in->c;
   p.x_batch = in->x_batch; p.x_token = in->x_token;
   p.dt_batch = in->dt_batch; p.dt_token = in->dt_token;

@@ -826,8 +826,13 @@ PyObject* selective_scan(PyObject* const* args, Py_ssize_t n) {
     return not_here();
   Guard guard(x->device().index());
   const cudaStream_t s = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  // a long call's scratch is its own (captured calls may be replayed side by side); timeouts show up in check_status
   Workspace ws;
-  if (T > 1 && !workspace(*x, s, g_lib.selective_scan_workspace_bytes(), &ws)) return nullptr;
+  at::Tensor scratch;
+  if (T >= 512) {
+    if (!workspace(*x, s, 4, &ws)) return nullptr;
+    scratch = empty({(int64_t)g_lib.selective_scan_workspace_bytes()}, at::kByte, x->device());
+  }
   at::Tensor y = empty({B, T, E}, x->scalar_type(), x->device());
   // (long calls hand states from chunk to chunk in it, whether it is returned or not)
   at::Tensor made = inplace ? *state : empty({B, E, N}, at::kFloat, x->device());
@@ -841,7 +846,9 @@ PyObject* selective_scan(PyObject* const* args, Py_ssize_t n) {
   in.a = fptr(a); in.d = fptr(d); in.dt_bias = fptr(bias);
   in.softplus = PyObject_IsTrue(args[10]) == 1;
   if (!succeeded(g_lib.selective_scan(&in, ptr(pos), pc, fptr(state), B, T, E, (int)G, (int)N, code, y.mutable_data_ptr(),
-                                      static_cast<float*>(made.mutable_data_ptr()), ws.ptr, ws.bytes, s)))
+                                      static_cast<float*>(made.mutable_data_ptr()),
+                                      scratch.defined() ? scratch.mutable_data_ptr() : nullptr,
+                                      scratch.defined() ? (size_t)scratch.numel() : 0, static_cast<int*>(ws.ptr), s)))
     return nullptr;
   return with_state(std::move(y), std::move(made), args[9], inplace, want);
 }

@@ -338,7 +338,6 @@ struct ConvArgs {
 };
 cudaError_t launch_causal_conv(const ConvArgs& p, int dtype, cudaStream_t s);
 
-struct WsHeader;
 // selective_scan.cu (strides in elements)
 struct SelectiveArgs {
   const void *x, *dt, *z, *b, *c;        // z: or NULL
@@ -352,7 +351,8 @@ struct SelectiveArgs {
   int groups, N;
   void* y;
   float* state_out;                      // or NULL
-  WsHeader* header;               // or NULL: time is not cut into chunks
+  unsigned* ticket;                      // scratch, or NULL: time is not cut into chunks
+  int* status;                           // or NULL
   int per_group, copy_x, copy_n, store4; // set by the launcher, like what follows
   int blocks_per_group;
   int64_t blocks, chunk, chunks;         // of channels; of time: length and number

@@ -133,7 +133,7 @@ template <typename T, int S_, int C_, int L_, int kTile_> struct Shape {
 
 // Waits until chunk - 1 of a block of channels has left its states.  The CTA that has drawn it is running (items are
 // drawn in this order by CTAs that have started), and none waits for a later one.
-__device__ __forceinline__ void wait_for(const int* done, int chunk, WsHeader* header) {
+__device__ __forceinline__ void wait_for(const int* done, int chunk, int* status) {
   if (threadIdx.x == 0) {
     int seen = 0;
     for (unsigned n = 0; n < kWaitLimit; ++n) {
@@ -141,7 +141,7 @@ __device__ __forceinline__ void wait_for(const int* done, int chunk, WsHeader* h
       if (seen >= chunk) break;
       __nanosleep(200);
     }
-    if (seen < chunk) atomicExch(&header->status, kStatusTimeout);
+    if (seen < chunk && status != nullptr) atomicExch(status, kStatusTimeout);
   }
   meet<kTeam>(kOwnersMeet);
 }
@@ -417,7 +417,7 @@ selective_scan_kernel(const SelectiveArgs p) {
       const int l = tid & (L - 1), owner = tid / L;
       auto channel_of = [&](int c) { const int at = owner + c * Sh::kOwners; return at % kQuads * 4 + at / kQuads; };
       auto state_of = [&](int s) { return s / kRun * kRun * L + l * kRun + s % kRun; };
-      if (chunk > 0) wait_for(p.done + block, (int)chunk, p.header);
+      if (chunk > 0) wait_for(p.done + block, (int)chunk, p.status);
       const float* from = chunk > 0 ? p.state_out : p.state_in;
       Pair h[C][S / 2], a2[C][S / 2];
 #pragma unroll
@@ -514,7 +514,7 @@ selective_scan_kernel(const SelectiveArgs p) {
         __threadfence();
         asm volatile("st.release.gpu.global.s32 [%0], %1;" :: "l"(p.done + block), "r"((int)chunk + 1) : "memory");
       }
-      s_item = (int)(atomicAdd(&p.header->ticket, 1u) + gridDim.x);
+      s_item = (int)(atomicAdd(p.ticket, 1u) + gridDim.x);
     }
     __syncthreads();
     item = s_item;
@@ -536,7 +536,7 @@ cudaError_t launch_kernel(SelectiveArgs p, cudaStream_t s) {
   if (p.blocks >= ((int64_t)1 << 31)) return cudaErrorInvalidValue;
   int64_t grid = p.blocks;
   // Chunks of time drawn by a ticket.
-  if (p.header != nullptr && p.state_out != nullptr && p.T >= 512) {
+  if (p.ticket != nullptr && p.state_out != nullptr && p.T >= 512) {
     int per_sm = 0;
     if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, selective_scan_kernel<T, Sh, kAligned>, 2 * kTeam,
                                                            Sh::kBytes)) != cudaSuccess) return e;
@@ -546,9 +546,8 @@ cudaError_t launch_kernel(SelectiveArgs p, cudaStream_t s) {
       // (24 of them: the last round is short of 4 % at most; no longer than a wait for one is given)
       p.chunk = min((int64_t)4096, max((int64_t)128, (p.T / 24 + Sh::kTile - 1) / Sh::kTile * Sh::kTile));
       p.chunks = (p.T + p.chunk - 1) / p.chunk;
-      p.done = reinterpret_cast<int*>(p.header + 1);
-      if ((e = cudaMemsetAsync(&p.header->ticket, 0, sizeof(WsHeader) - sizeof(int) + p.blocks * sizeof(int), s)) != cudaSuccess)
-        return e;
+      p.done = reinterpret_cast<int*>(p.ticket) + 1;
+      if ((e = cudaMemsetAsync(p.ticket, 0, (1 + p.blocks) * sizeof(int), s)) != cudaSuccess) return e;
     }
   }
   selective_scan_kernel<T, Sh, kAligned><<<(unsigned)grid, 2 * kTeam, Sh::kBytes, s>>>(p);
@@ -898,7 +897,7 @@ int copy_bytes(const void* base, int64_t batch, int64_t token, int64_t width, in
 
 }  // namespace
 
-size_t selective_workspace_bytes() { return sizeof(WsHeader) + kMostBlocks * sizeof(int); }
+size_t selective_workspace_bytes() { return (1 + kMostBlocks) * sizeof(int); }
 
 cudaError_t launch_selective_scan(SelectiveArgs p, int dtype, cudaStream_t s) {
   if (p.B == 0 || p.E == 0) return cudaSuccess;

@@ -365,11 +365,11 @@ def test_refusals_of_the_library():
 
   def scan(b=1, t=4, e=8, groups=1, n=16, dtype=1, y=16, ws=(None, 0), **of):
     p = _lib.RgkScanInputs(**{**{k: 16 for k in ("x", "dt", "b", "c", "a")}, **of})
-    return lib.rgk_selective_scan(ctypes.byref(p), None, 0, None, b, t, e, groups, n, dtype, y, None, *ws, None)
+    return lib.rgk_selective_scan(ctypes.byref(p), None, 0, None, b, t, e, groups, n, dtype, y, None, *ws, None, None)
   assert scan(x=None) == scan(a=None) == scan(c=None) == scan(y=None) == scan(dtype=7) == scan(t=-1) == -1
   assert scan(n=0) == scan(n=257) == scan(groups=3) == scan(groups=0) == scan(b=70000) == -2
   assert b"70000" in lib.rgk_last_error()
   assert scan(x=17) == scan(a=18) == scan(d=18) == -3
-  assert scan(ws=(256, lib.rgk_selective_scan_workspace_bytes() - 1)) == -6 and scan(ws=(64, 1 << 30)) == -3
-  assert lib.rgk_selective_scan(None, None, 0, None, 1, 4, 8, 1, 16, 1, 16, None, None, 0, None) == -1
+  assert scan(ws=(256, lib.rgk_selective_scan_workspace_bytes() - 1)) == -6 and scan(ws=(66, 1 << 30)) == -3
+  assert lib.rgk_selective_scan(None, None, 0, None, 1, 4, 8, 1, 16, 1, 16, None, None, 0, None, None) == -1
   assert scan(b=0) == scan(t=0) == scan(e=0) == 0
