@@ -117,6 +117,23 @@ def test_captured_prompts_on_two_streams():
 
 
 @pytest.mark.gpu
+def test_long_calls_on_two_streams_at_once():
+  import recurrentgemma_b200 as rg
+  from tests.test_state_space import scan_case
+  cases = [scan_case(seed, 4, 700, 5120, 16, torch.bfloat16) for seed in (5, 6)]
+  want = [rg.selective_scan(**c) for c in cases]
+  streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+  torch.cuda.synchronize()
+  for _ in range(5):
+    got = []
+    for c, stream in zip(cases, streams):
+      with torch.cuda.stream(stream):
+        got.append(rg.selective_scan(**c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for g, w in zip(got, want) for p, q in zip(g, w))
+
+
+@pytest.mark.gpu
 def test_left_padded_batch():
   """Rows of a padded batch (padding at positions of -1, the first token at 0) give what they give alone."""
   m = Layers(dtype=torch.float32)

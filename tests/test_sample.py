@@ -24,7 +24,8 @@ def definition(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
     w = torch.exp((values - values[0]) / t)
     w[values == values[0]] = 1.0
     w[values == -math.inf] = 0.0
-    w = torch.round(w * 2.0 ** 44) / 2.0 ** 44
+    unit = 2.0 ** (44 if len(l) <= 2 ** 18 else 43 if len(l) <= 2 ** 19 else 42)
+    w = torch.round(w * unit) / unit
     if k > 0:
       w[k:] = 0.0
     if p < 1.0:
@@ -87,6 +88,15 @@ def test_sample_large_vocabulary(m, dtype):
   for i in list(some)[:6]:
     alone = rg.sample(logits[i:i + 1], uniforms[i:i + 1], **{k: v[i:i + 1] for k, v in settings.items()})
     assert torch.equal(alone, got[i:i + 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [2 ** 18, 2 ** 18 + 1, 2 ** 20])
+def test_sample_largest_vocabularies(v):
+  import recurrentgemma_b200 as rg
+  logits, uniforms, _ = rows(v, 2, v, torch.float32)
+  for settings in ({}, dict(top_k=100, top_p=0.9), dict(temperature=30.0, top_p=0.5), dict(top_k=v // 4, top_p=0.9)):
+    assert torch.equal(rg.sample(logits, uniforms, **settings), definition(logits, uniforms, **settings)), settings
 
 
 @pytest.mark.gpu
