@@ -564,8 +564,7 @@ cudaError_t launch(const SelectiveArgs& p, cudaStream_t s) {
 
 // One time step: the states are read and written once and bound it.  A lane holds four states (8 beyond 128) of each
 // of kRows sequences, L lanes a channel, so that a, d and the bias are read once for kRows sequences and all that is
-// read of kRows sequences is in flight at a time.  kVec: states, b and c are read and written four at a time.  256 x 5120
-// x 16 in bfloat16: 48 us.
+// read of kRows sequences is in flight at a time.  kVec: states, b and c are read and written four at a time.
 __device__ __forceinline__ float softplus_step(float v) {        // softplus_steps for one
   const float e = exp2_fast(-fabsf(v) * kLog2e);
   float q = softplus_coefficient(9);
@@ -796,23 +795,29 @@ cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
                    fits(p.c, p.c_batch, sizeof(T));
   const unsigned across = (unsigned)((p.E + 256 / L - 1) / (256 / L));
   if constexpr (S == 4) {
-    static PerDeviceOnce once;
-    int sms = 0;
-    const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
-    if (e != cudaSuccess) return e;
-    // eight sequences a thread and more where four CTAs an SM have that many
-    const int64_t down = max((int64_t)1, (int64_t)4 * sms / across), per = (p.B + down - 1) / down;
-    if (vec && per >= 8) {
-      selective_steps_kernel<T, L><<<dim3(across, (unsigned)((p.B + per - 1) / per)), 256, 0, s>>>(p, (int)per);
+    if (vec) {
+      static PerDeviceOnce once;
+      int sms = 0;
+      const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
+      if (e != cudaSuccess) return e;
+      // eight sequences a thread and more where four CTAs an SM have that many
+      const int64_t down = max((int64_t)1, (int64_t)4 * sms / across), per = (p.B + down - 1) / down;
+      if (per >= 8)
+        selective_steps_kernel<T, L><<<dim3(across, (unsigned)((p.B + per - 1) / per)), 256, 0, s>>>(p, (int)per);
+      else
+        selective_step_kernel<T, S, L, 1, true><<<dim3(across, (unsigned)p.B), 256, 0, s>>>(p);
       return cudaGetLastError();
     }
   }
   // four sequences a thread where they still give every SM its threads
   const bool many = across * p.B >= 4 * 8 * 148;
   const dim3 grid(across, (unsigned)(many ? (p.B + 3) / 4 : p.B));
-  if (many && vec) selective_step_kernel<T, S, L, 4, true><<<grid, 256, 0, s>>>(p);
-  else if (many) selective_step_kernel<T, S, L, 4, false><<<grid, 256, 0, s>>>(p);
-  else if (vec) selective_step_kernel<T, S, L, 1, true><<<grid, 256, 0, s>>>(p);
+  if constexpr (S != 4) {
+    if (vec && many) selective_step_kernel<T, S, L, 4, true><<<grid, 256, 0, s>>>(p);
+    else if (vec) selective_step_kernel<T, S, L, 1, true><<<grid, 256, 0, s>>>(p);
+    if (vec) return cudaGetLastError();
+  }
+  if (many) selective_step_kernel<T, S, L, 4, false><<<grid, 256, 0, s>>>(p);
   else selective_step_kernel<T, S, L, 1, false><<<grid, 256, 0, s>>>(p);
   return cudaGetLastError();
 }

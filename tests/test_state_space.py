@@ -182,6 +182,7 @@ SCAN = [
     (131, 1, 300, 130, 1, 0, dict(z=False)),
     (256, 1, 5120, 16, 1, 2, {}),                  # many sequences a thread
     (300, 1, 5132, 8, 2, 0, dict(state=False)),
+    (256, 1, 5120, 7, 1, 0, {}), (256, 1, 200, 200, 1, 0, {}),         # the same without vectors, with eight states a lane
     (1, 2, 8, 1, 1, 0, {}),
     (2, 31, 64, 16, 2, 7, {}),
     (2, 32, 36, 16, 1, 0, dict(state=False)),
