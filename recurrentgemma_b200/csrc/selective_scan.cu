@@ -562,9 +562,6 @@ cudaError_t launch(const SelectiveArgs& p, cudaStream_t s) {
   return aligned ? launch_kernel<T, Sh, true>(p, s) : launch_kernel<T, Sh, false>(p, s);
 }
 
-// One time step: the states are read and written once and bound it.  A lane holds four states (8 beyond 128) of each
-// of kRows sequences, L lanes a channel, so that a, d and the bias are read once for kRows sequences and all that is
-// read of kRows sequences is in flight at a time.  kVec: states, b and c are read and written four at a time.
 __device__ __forceinline__ float softplus_step(float v) {        // softplus_steps for one
   const float e = exp2_fast(-fabsf(v) * kLog2e);
   float q = softplus_coefficient(9);
@@ -581,6 +578,9 @@ __device__ __forceinline__ void widen4(const uint2& v, float* f) {
   f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
 }
 
+// One time step: the states are read and written once and bound it.  A lane holds four states (8 beyond 128) of each
+// of kRows sequences, L lanes a channel, so that a, d and the bias are read once for kRows sequences and all that is
+// read of kRows sequences is in flight at a time.  kVec: states, b and c are read and written four at a time.
 template <typename T, int S, int L, int kRows, bool kVec>
 __global__ void __launch_bounds__(256)
 selective_step_kernel(const SelectiveArgs p) {
