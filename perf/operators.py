@@ -117,7 +117,8 @@ def prepare(case, seed):
     # a broad bulk and some tens of likely tokens a row, capped as the model caps its logits
     logits = normal(m, v, std=2.0, dtype=torch.float32)
     likely = torch.randint(0, v, (m, 64), generator=g, device="cuda")
-    logits.scatter_(1, likely, 4.0 + 10.0 * uniform(m, 64))
+    # (where two of them are one token, the larger value: inputs of one seed are the same each time)
+    logits.scatter_reduce_(1, likely, 4.0 + 10.0 * uniform(m, 64), "amax", include_self=False)
     s["logits"] = (30.0 * torch.tanh(logits / 30.0)).to(dt)
     s["uniforms"] = uniform(m)
     settings = {n: case[n] for n in ("temperature", "top_k", "top_p", "min_p")}
