@@ -131,8 +131,9 @@ template <typename T, int S_, int C_, int L_, int kTile_> struct Shape {
   static_assert(kChan % 4 == 0 && kTile <= 32 && kTile % kUnroll == 0 && kBytes <= 227 * 1024, "a tile");
 };
 
-// Waits until chunk - 1 of a block of channels has left its states.  The CTA that has drawn it is running (items are
-// drawn in this order by CTAs that have started), and none waits for a later one.
+// Waits until chunk - 1 of a block of channels has left its states.  The CTA that has drawn it is running (all items are
+// drawn in this order, the first one of a CTA too, by CTAs that have started), and none waits for a later one: however
+// few of the CTAs find a place on the device, the item that was drawn first among the unfinished ones goes on.
 __device__ __forceinline__ void wait_for(const int* done, int chunk, int* status) {
   if (threadIdx.x == 0) {
     int seen = 0;
@@ -173,8 +174,13 @@ selective_scan_kernel(const SelectiveArgs p) {
     __syncthreads();
   }
 
+  auto draw = [&]() -> int64_t {                                 // for all of the CTA; what it has done is published
+    if (threadIdx.x == 0) s_item = (int)atomicAdd(p.ticket, 1u);
+    __syncthreads();
+    return s_item;
+  };
   const int64_t items = p.chunks * p.blocks;
-  for (int64_t item = blockIdx.x; item < items;) {
+  for (int64_t item = p.chunks == 1 ? blockIdx.x : draw(); item < items;) {
     const int64_t chunk = item / p.blocks;
     const int block = (int)(item - chunk * p.blocks);
     const int per_row = p.groups * p.blocks_per_group;
@@ -514,10 +520,8 @@ selective_scan_kernel(const SelectiveArgs p) {
         __threadfence();
         asm volatile("st.release.gpu.global.s32 [%0], %1;" :: "l"(p.done + block), "r"((int)chunk + 1) : "memory");
       }
-      s_item = (int)(atomicAdd(p.ticket, 1u) + gridDim.x);
     }
-    __syncthreads();
-    item = s_item;
+    item = draw();
   }
 }
 
