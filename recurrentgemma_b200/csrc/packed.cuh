@@ -42,28 +42,28 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x of a pair on the multiply-add pipe: x = n + f with n from the low bits of a sum with 1.5 2^23 (+ 127, so that they
-// are an exponent), 2^f as a polynomial of degree 5 with constant term 1, fitted on [-1/2, 1/2] for the smallest largest
-// relative error (9.1e-8; 1.6e-7 in float32 arithmetic, and on average none near 0, where the hardware's exponential
-// is 2e-8 too small).  Infinite from 2^128, zero below 2^-126; a NaN stays one.
+// 2^x of a pair on the multiply-add pipe: x = n + f with n from the low bits of a sum with 1.5 2^23 (+ 126, so that they
+// are the exponent of 2^(n-1)), times 2^(f+1) as a polynomial of degree 5 with constant term 2, fitted on [-1/2, 1/2] for the
+// smallest largest relative error (9.1e-8; 1.6e-7 in float32 arithmetic, and on average none near 0, where the hardware's
+// exponential is 2e-8 too small).  Infinite from 2^128, zero below 2^-125.5; a NaN stays one.
 __device__ __forceinline__ float exponent_range(float v) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(-127.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(-126.0f));
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(r) : "f"(128.0f));
   return r;
 }
 __device__ __forceinline__ Pair exp2_poly(Pair x) {
-  constexpr float kMagic = 12583039.0f;
+  constexpr float kMagic = 12583038.0f;
   const float2 v = split(x);
   x = pair(exponent_range(v.x), exponent_range(v.y));
   const Pair r = add2(x, pair(kMagic, kMagic));
   const Pair f = add2(x, fma2(r, pair(-1.0f, -1.0f), pair(kMagic, kMagic)));
-  Pair q = pair(0.001326472731307149f, 0.001326472731307149f);
-  q = fma2(q, f, pair(0.009671512991189957f, 0.009671512991189957f));
-  q = fma2(q, f, pair(0.05550733581185341f, 0.05550733581185341f));
-  q = fma2(q, f, pair(0.24022242426872253f, 0.24022242426872253f));
-  q = fma2(q, f, pair(0.6931470036506653f, 0.6931470036506653f));
-  q = fma2(q, f, pair(1.0f, 1.0f));
+  Pair q = pair(0.002652945462614298f, 0.002652945462614298f);
+  q = fma2(q, f, pair(0.019343025982379913f, 0.019343025982379913f));
+  q = fma2(q, f, pair(0.11101467162370682f, 0.11101467162370682f));
+  q = fma2(q, f, pair(0.48044484853744507f, 0.48044484853744507f));
+  q = fma2(q, f, pair(1.3862940073013306f, 1.3862940073013306f));
+  q = fma2(q, f, pair(2.0f, 2.0f));
   const float2 n = split(r);
   return mul2(q, pair(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23)));
 }
