@@ -35,16 +35,22 @@ constexpr unsigned kWaitLimit = 1u << 23;                       // polls, 0.2 us
 
 // softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1]: log1p(e) / e by a polynomial fitted for the
 // smallest largest relative error on [0, 1] (5e-9; 1.8e-7 in float32 arithmetic).  Steps of 1e-3 come out with their
-// relative precision, which the hardware logarithm of 1 + e would lose.  (A NaN stays one: e is.)
+// relative precision, which the hardware logarithm of 1 + e would lose.  (A NaN stays one: e is.)  kExact: e by exp_poly,
+// for float32; the hardware's exponential of |v| log2(e) is 1.5e-7 off on average for steps of 1e-3 to 1.
 constexpr float softplus_coefficient(int i) {
   constexpr float k[10] = {1.0f, -0.4999990165233612f, 0.3332996368408203f, -0.24954134225845337f,
                            0.1967593878507614f, -0.15305590629577637f, 0.10603651404380798f,
                            -0.056959498673677444f, 0.01985144428908825f, -0.0032440212089568377f};
   return k[i];
 }
+template <bool kExact>
 __device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
-  const float2 arg = split(mul2(pair(fabsf(v0), fabsf(v1)), pair(-kLog2e, -kLog2e)));
-  const Pair e = pair(exp2_fast(arg.x), exp2_fast(arg.y));
+  Pair e;
+  if constexpr (kExact) {
+    e = exp_poly(-fabsf(v0), -fabsf(v1));
+  } else {
+    e = exp2_pair(mul2(pair(fabsf(v0), fabsf(v1)), pair(-kLog2e, -kLog2e)));
+  }
   Pair p = pair(softplus_coefficient(9), softplus_coefficient(9));
 #pragma unroll
   for (int i = 8; i >= 0; --i) p = fma2(p, e, pair(softplus_coefficient(i), softplus_coefficient(i)));
@@ -324,7 +330,7 @@ selective_scan_kernel(const SelectiveArgs p) {
           if (p.softplus) {
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-              const float2 two = softplus_steps(step[i], step[i + 1]);
+              const float2 two = softplus_steps<sizeof(T) == 4>(step[i], step[i + 1]);
               step[i] = two.x; step[i + 1] = two.y;
             }
           }
@@ -417,7 +423,7 @@ selective_scan_kernel(const SelectiveArgs p) {
       constexpr int kRun = S < 4 ? S : 4, kUnroll = Sh::kUnroll;
       // In float32, and up to 4 states, where there is room for it, the decays are polynomials: slow states keep their
       // terms for a thousand steps, and that the hardware's exponential is a little small shows in them (2048 steps of
-      // one state: the states are 1.2e-6 off 64 bits with it, 2.8e-7 with the polynomial, which takes 6 % longer there
+      // one state: the states are 1.2e-6 off 64 bits with it, 2.2e-7 with the polynomial, which takes 6 % longer there
       // and 20 to 30 % with 8 states).
       constexpr bool kExact = sizeof(T) == 4 || Sh::kPad <= 4;
       const int l = tid & (L - 1), owner = tid / L;
@@ -658,7 +664,7 @@ selective_step_kernel(const SelectiveArgs p) {
     if (b >= p.B) break;
     const float xr = static_cast<float>(x[r]);
     float now = static_cast<float>(dt[r]) + bias;
-    if (p.softplus) now = softplus_steps(now, now).x;
+    if (p.softplus) now = softplus_steps<false>(now, now).x;
     const float put = now * xr;
     float sum = 0.0f;
 #pragma unroll

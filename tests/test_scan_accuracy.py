@@ -27,3 +27,91 @@ def test_growth_up_to_the_largest_float(t, n, dtype):
   assert (want < torch.finfo(torch.float32).max).all()
   assert torch.isfinite(got).all()
   assert ((got.double() - want).abs() <= (3 * 88.8 + 8) * U * want).all()
+
+
+def off(got, want):
+  """Relative to 64 bits, in the 2-norm."""
+  return ((got.double() - want).norm() / want.norm()).item()
+
+
+def off_each(got, want):
+  """Relative to each value in 64 bits, root mean square."""
+  return ((got.double() - want) / want).square().mean().sqrt().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [2, 33])
+def test_steps_in_float32(t):
+  """Steps softplus(dt) of 1e-4 to 0.3, seen in states that forget all else: the exponential (0.45 u rms), the logarithm
+  (0.7 u) and two products (0.42 u each) make 1.0 u; half as much again is allowed."""
+  import recurrentgemma_b200 as rg
+  g = torch.Generator(device="cuda").manual_seed(t)
+  e, n = 2560, 16
+  dt = -1.0 - 8.0 * torch.rand((1, t, e), generator=g, device="cuda")
+  x = torch.randn((1, t, e), generator=g, device="cuda")
+  b, c = (torch.randn((1, t, 1, n), generator=g, device="cuda") for _ in range(2))
+  a = torch.full((e, n), -1e7, device="cuda")
+  got = rg.selective_scan(x, dt, a, b, c)[1]
+  want = (torch.log1p(torch.exp(dt[:, -1].double())) * x[:, -1].double())[:, :, None] * b[:, -1].double()
+  assert off_each(got, want) <= 1.5 * U
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [4, 16, 21])
+def test_decay_factors_in_float32(n):
+  """States whose decay factors are 1/2 to 1.  A term of k steps ago has passed k factors and k multiply-adds, and weighs
+  with the square of its decay: 1.4 steps on average.  So of the squares of the errors (rms, in u) 1.4 times a factor's
+  (0.45 the exponential, 0.2 each the argument and the rate times log2(e)) and a multiply-add's (0.42), and once those of the
+  two products that a term is (0.42): 1.0 u in all.  A fifth more is allowed."""
+  import recurrentgemma_b200 as rg
+  g = torch.Generator(device="cuda").manual_seed(n)
+  t, e = 40, 2560
+  dt = math.log(2.0) * torch.rand((1, t, e), generator=g, device="cuda")
+  x = torch.randn((1, t, e), generator=g, device="cuda")
+  b = torch.randn((1, t, 1, n), generator=g, device="cuda")
+  a = torch.full((e, n), -1.0, device="cuda")
+  got = rg.selective_scan(x, dt, a, b, b, softplus=False)[1]
+  want = torch.zeros((1, e, n), dtype=torch.float64, device="cuda")
+  for i in range(t):
+    step = dt[:, i].double()
+    want = torch.exp(-step)[:, :, None] * want + (step * x[:, i].double())[:, :, None] * b[:, i].double()
+  assert off(got, want) <= 1.2 * U
+
+
+def layer(seed, b, t, e, n, dtype, gate=True):
+  """Steps of 1e-3 to 1e-1, decay rates of about 1 to n, as trained layers have them."""
+  g = torch.Generator(device="cuda").manual_seed(seed)
+  normal = lambda *s: torch.randn(s, generator=g, device="cuda")                 # noqa: E731
+  step = torch.exp(torch.rand(e, generator=g, device="cuda") * math.log(100.0) + math.log(1e-3))
+  return dict(x=normal(b, t, e).to(dtype), dt=(0.5 * normal(b, t, e)).to(dtype),
+              a=-(torch.arange(1, n + 1, device="cuda") * torch.exp(0.2 * normal(e, n))),
+              b=normal(b, t, 1, n).to(dtype), c=normal(b, t, 1, n).to(dtype), d=0.5 * normal(e),
+              z=normal(b, t, e).to(dtype) if gate else None, dt_bias=step + torch.log(-torch.expm1(-step)))
+
+
+def token_by_token(case, dtype):
+  """The formula in `dtype`, a token after the other: (y, state)."""
+  x, dt, a, b, c, d, z, bias = (None if case[k] is None else case[k].to(dtype)
+                                for k in ("x", "dt", "a", "b", "c", "d", "z", "dt_bias"))
+  step = dt + bias
+  step = torch.where(step > 0, step, 0.0) + torch.log1p(torch.exp(-step.abs()))
+  h = x.new_zeros(x.shape[0], *a.shape)
+  y = torch.empty_like(x)
+  for i in range(x.shape[1]):
+    now = step[:, i, :, None]
+    h = torch.exp(now * a) * h + now * x[:, i, :, None] * b[:, i]
+    y[:, i] = (h * c[:, i]).sum(-1) + d * x[:, i]
+  return (y if z is None else y * (z / (1.0 + torch.exp(-z)))), h
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 8, 16, 21, 48])
+@pytest.mark.parametrize("gate", [True, False])
+def test_sequences_in_float32_are_as_exact_as_the_formula(n, gate):
+  """No further from 64 bits, outputs and states, than the formula in float32 with its library's functions."""
+  import recurrentgemma_b200 as rg
+  case = layer(n, 2, 700, 320, n, torch.float32, gate)
+  want, plain = token_by_token(case, torch.float64), token_by_token(case, torch.float32)
+  got = rg.selective_scan(**case)
+  for k, p, w in zip(got, plain, want):
+    assert off(k, w) <= off(p, w)
