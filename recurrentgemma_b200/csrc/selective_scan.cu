@@ -35,7 +35,7 @@ constexpr unsigned kWaitLimit = 1u << 23;                       // polls, 0.2 us
 
 // softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1]: log1p(e) / e by a polynomial fitted for the
 // smallest largest relative error on [0, 1] (5e-9; 1.8e-7 in float32 arithmetic).  Steps of 1e-3 come out with their
-// relative precision, which the hardware logarithm of 1 + e would lose.  (A NaN stays one: e is.)  kExact: e by exp_poly,
+// relative precision, which the hardware logarithm of 1 + e would lose.  (A NaN stays one: e is.)  kExact: e by exp_exact,
 // for float32; the hardware's exponential of |v| log2(e) is 1.5e-7 off on average for steps of 1e-3 to 1.
 constexpr float softplus_coefficient(int i) {
   constexpr float k[10] = {1.0f, -0.4999990165233612f, 0.3332996368408203f, -0.24954134225845337f,
@@ -47,7 +47,7 @@ template <bool kExact>
 __device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
   Pair e;
   if constexpr (kExact) {
-    e = exp_poly(-fabsf(v0), -fabsf(v1));
+    e = pair(exp_exact(-fabsf(v0)), exp_exact(-fabsf(v1)));
   } else {
     e = exp2_pair(mul2(pair(fabsf(v0), fabsf(v1)), pair(-kLog2e, -kLog2e)));
   }
@@ -55,6 +55,18 @@ __device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
 #pragma unroll
   for (int i = 8; i >= 0; --i) p = fma2(p, e, pair(softplus_coefficient(i), softplus_coefficient(i)));
   return split(fma2(p, e, pair(fmaxf(v0, 0.0f), fmaxf(v1, 0.0f))));
+}
+
+// In float32, and up to 4 states (of a channel, rounded up), the decays are exp2_exact: slow states keep their terms for a
+// thousand steps, and that the hardware's exponential is a little small shows in them.  2048 steps of 1 / 8 / 16 states in
+// float32: 1.2e-6 / 7.8e-7 / 6.0e-7 off 64 bits with it, 2.1e-7 / 1.7e-7 / 1.5e-7 so, for 2 / 5 / 24 % more time (a step of
+// 256 sequences 45 -> 48 us).  bfloat16 calls of more states keep the hardware's: 16 of them 6.1e-7 off, where 1.4e-7
+// would take 30 % longer.  One rule for sequences and single steps, so that they come to the same states.
+template <typename T> constexpr bool exact_decays(int states) { return sizeof(T) == 4 || states <= 4; }
+// 2^(step a) for two states
+template <bool kExact> __device__ __forceinline__ float2 decays(float step, float a0, float a1) {
+  const Pair arg = mul2(pair(step, step), pair(a0, a1));
+  return split(kExact ? exp2_exact(arg) : exp2_pair(arg));
 }
 
 // four consecutive elements, at an address aligned to four of them
@@ -421,11 +433,7 @@ selective_scan_kernel(const SelectiveArgs p) {
       // A thread's channels, for each of its c the one at place owner + c * kOwners, and their states in runs of kRun
       // that lie next to its neighbours' (value kRun r + i is state kRun L r + kRun l + i).
       constexpr int kRun = S < 4 ? S : 4, kUnroll = Sh::kUnroll;
-      // In float32, and up to 4 states, where there is room for it, the decays are polynomials: slow states keep their
-      // terms for a thousand steps, and that the hardware's exponential is a little small shows in them (2048 steps of
-      // one state: the states are 1.2e-6 off 64 bits with it, 2.2e-7 with the polynomial, which takes 6 % longer there
-      // and 20 to 30 % with 8 states).
-      constexpr bool kExact = sizeof(T) == 4 || Sh::kPad <= 4;
+      constexpr bool kExact = exact_decays<T>(Sh::kPad);
       const int l = tid & (L - 1), owner = tid / L;
       auto channel_of = [&](int c) { const int at = owner + c * Sh::kOwners; return at % kQuads * 4 + at / kQuads; };
       auto state_of = [&](int s) { return s / kRun * kRun * L + l * kRun + s % kRun; };
@@ -487,7 +495,7 @@ selective_scan_kernel(const SelectiveArgs p) {
                   const Pair arg = mul2(step2, a2[c][s]);
                   Pair before = h[c][s];
                   if (decltype(with_starts)::value && ((starts >> t) & 1u)) before = 0;
-                  h[c][s] = fma2(kExact ? exp2_poly(arg) : exp2_pair(arg), before, mul2(put2, vb[s]));
+                  h[c][s] = fma2(kExact ? exp2_exact(arg) : exp2_pair(arg), before, mul2(put2, vb[s]));
                   both = s == 0 ? mul2(h[c][s], vc[s]) : fma2(h[c][s], vc[s], both);
                 }
                 const float2 halves = split(both);
@@ -572,8 +580,9 @@ cudaError_t launch(const SelectiveArgs& p, cudaStream_t s) {
   return aligned ? launch_kernel<T, Sh, true>(p, s) : launch_kernel<T, Sh, false>(p, s);
 }
 
+template <bool kExact>
 __device__ __forceinline__ float softplus_step(float v) {        // softplus_steps for one
-  const float e = exp2_fast(-fabsf(v) * kLog2e);
+  const float e = kExact ? exp_exact(-fabsf(v)) : exp2_fast(-fabsf(v) * kLog2e);
   float q = softplus_coefficient(9);
 #pragma unroll
   for (int i = 8; i >= 0; --i) q = fmaf(q, e, softplus_coefficient(i));
@@ -596,6 +605,7 @@ __global__ void __launch_bounds__(256)
 selective_step_kernel(const SelectiveArgs p) {
   using Raw = typename Four<T>::type;
   constexpr int Q = S / 4;
+  constexpr bool kExact = exact_decays<T>(S * L);
   const int64_t at = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
   const int l = threadIdx.x % L;
   const bool in = at < p.E;
@@ -664,7 +674,7 @@ selective_step_kernel(const SelectiveArgs p) {
     if (b >= p.B) break;
     const float xr = static_cast<float>(x[r]);
     float now = static_cast<float>(dt[r]) + bias;
-    if (p.softplus) now = softplus_steps<false>(now, now).x;
+    if (p.softplus) now = softplus_step<sizeof(T) == 4>(now);
     const float put = now * xr;
     float sum = 0.0f;
 #pragma unroll
@@ -675,9 +685,12 @@ selective_step_kernel(const SelectiveArgs p) {
       widen4(vc[r][k], fc);
       widen4(h[r][k], fh);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fh[i] = fmaf(exp2_fast(now * a2[4 * k + i]), fh[i], put * fb[i]);
+      for (int i = 0; i < 4; i += 2) {
+        const float2 decay = decays<kExact>(now, a2[4 * k + i], a2[4 * k + i + 1]);
+        fh[i] = fmaf(decay.x, fh[i], put * fb[i]);
+        fh[i + 1] = fmaf(decay.y, fh[i + 1], put * fb[i + 1]);
         sum = fmaf(fh[i], fc[i], sum);
+        sum = fmaf(fh[i + 1], fc[i + 1], sum);
       }
       if (p.state_out != nullptr && in) {
         float* to = p.state_out + (b * p.E + e) * p.N + n;
@@ -711,6 +724,7 @@ __global__ void __launch_bounds__(256, 4)
 selective_steps_kernel(const SelectiveArgs p, int per) {
   using Raw = typename Four<T>::type;
   constexpr int kDepth = 8;
+  constexpr bool kExact = exact_decays<T>(4 * L);
   __shared__ float4 ring[kDepth][256];
   const int64_t at = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
   const int l = threadIdx.x % L;
@@ -772,13 +786,16 @@ selective_steps_kernel(const SelectiveArgs p, int per) {
     widen4(v.c, fc);
     const float x = static_cast<float>(v.x);
     float now = static_cast<float>(v.dt) + bias;
-    if (p.softplus) now = softplus_step(now);
+    if (p.softplus) now = softplus_step<sizeof(T) == 4>(now);
     const float put = now * x;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h[i] = fmaf(exp2_fast(now * a2[i]), h[i], put * fb[i]);
+    for (int i = 0; i < 4; i += 2) {
+      const float2 decay = decays<kExact>(now, a2[i], a2[i + 1]);
+      h[i] = fmaf(decay.x, h[i], put * fb[i]);
+      h[i + 1] = fmaf(decay.y, h[i + 1], put * fb[i + 1]);
       sum = fmaf(h[i], fc[i], sum);
+      sum = fmaf(h[i + 1], fc[i + 1], sum);
     }
     if (to != nullptr) {
       *reinterpret_cast<float4*>(to) = make_float4(h[0], h[1], h[2], h[3]);

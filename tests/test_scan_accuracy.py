@@ -115,3 +115,23 @@ def test_sequences_in_float32_are_as_exact_as_the_formula(n, gate):
   got = rg.selective_scan(**case)
   for k, p, w in zip(got, plain, want):
     assert off(k, w) <= off(p, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,b,t,e,n", [
+    (torch.float32, 2, 700, 320, 1), (torch.float32, 2, 700, 320, 16), (torch.float32, 2, 700, 320, 21),
+    (torch.float32, 1, 300, 40, 200), (torch.bfloat16, 2, 700, 320, 3), (torch.bfloat16, 2, 700, 320, 4),
+    (torch.float32, 64, 60, 5120, 16), (torch.bfloat16, 300, 60, 5120, 4)])         # (many sequences a thread)
+def test_single_steps_are_as_exact_as_the_formula(dtype, b, t, e, n):
+  """Steps that overwrite their state, one after the other: states, and float32 outputs, no further from 64 bits than the
+  formula in float32; the same rule as for a sequence in one call."""
+  import recurrentgemma_b200 as rg
+  case = layer(n + t, b, t, e, n, dtype)
+  want, plain = token_by_token(case, torch.float64), token_by_token(case, torch.float32)
+  state, y = torch.zeros(b, e, n, device="cuda"), torch.empty_like(case["x"])
+  for i in range(t):
+    now = {k: v[:, i:i + 1] if k in ("x", "dt", "b", "c", "z") else v for k, v in case.items()}
+    y[:, i:i + 1] = rg.selective_scan(**now, state=state, inplace=True)[0]
+  assert off(state, want[1]) <= off(plain[1], want[1])
+  if dtype == torch.float32:
+    assert off(y, want[0]) <= off(plain[0], want[0])
