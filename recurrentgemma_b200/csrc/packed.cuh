@@ -61,20 +61,40 @@ __device__ __forceinline__ Pair exp2_exact(Pair x) {
   const float2 v = split(x), near = split(q), far = split(exp2_pair(x));
   return pair(fabsf(v.x) <= 0.5f ? near.x : far.x, fabsf(v.y) <= 0.5f ? near.y : far.y);
 }
-// e^v by the hardware's exponential, with what rounding v log2(e) has left out put back (1e-7 of e^-7 without).
+// e^v by the hardware's exponential, with what rounding v log2(e) has left out put back (1e-7 of e^-7 without).  Zero below
+// -104, and as of 88 above it.
+constexpr float kLog2eLow = 1.92596299e-8f, kLn2 = 0.69314718056f;              // log2(e) - kLog2e
+__device__ __forceinline__ float exp_bounded(float v) {          // (no differences of infinities; a NaN stays one)
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(-104.0f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(88.0f));
+  return v;
+}
 __device__ __forceinline__ float exp_exact(float v) {
-  constexpr float kLog2eLow = 1.92596299e-8f, kLn2 = 0.69314718056f;            // log2(e) - kLog2e
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(-104.0f));      // (zero from there on; no difference of infinities)
+  v = exp_bounded(v);
   const float arg = v * kLog2e, r = exp2_fast(arg);
   return fmaf(r, kLn2 * fmaf(v, kLog2eLow, fmaf(v, kLog2e, -arg)), r);
 }
+__device__ __forceinline__ Pair exp_exact(float v0, float v1) {
+  const Pair v = pair(exp_bounded(v0), exp_bounded(v1)), log2e = pair(kLog2e, kLog2e);
+  const Pair arg = mul2(v, log2e), r = exp2_pair(arg);
+  const Pair low = fma2(v, pair(kLog2eLow, kLog2eLow), fma2(v, log2e, mul2(arg, pair(-1.0f, -1.0f))));
+  return fma2(r, mul2(low, pair(kLn2, kLn2)), r);
+}
 
-__device__ __forceinline__ float2 silu_fast(float v0, float v1) {
-  const float2 arg = split(mul2(pair(v0, v1), pair(-kLog2e, -kLog2e)));
-  float r0, r1;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(1.0f + exp2_fast(arg.x)));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(1.0f + exp2_fast(arg.y)));
-  return split(mul2(pair(v0, v1), pair(r0, r1)));
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// silu by the hardware's exponential and reciprocal, of a pair or of one; kExact: with exp_exact, 1.1 units of 2^-24 off on
+// average whatever the size of v (without, 1.1 for v of N(0, 1) and 3.8 for v of up to 20).
+template <bool kExact = false> __device__ __forceinline__ float2 silu_fast(float v0, float v1) {
+  const Pair e = kExact ? exp_exact(-v0, -v1) : exp2_pair(mul2(pair(v0, v1), pair(-kLog2e, -kLog2e)));
+  const float2 below = split(add2(e, pair(1.0f, 1.0f)));
+  return split(mul2(pair(v0, v1), pair(rcp_fast(below.x), rcp_fast(below.y))));
+}
+template <bool kExact> __device__ __forceinline__ float silu_fast(float v) {
+  return v * rcp_fast(1.0f + (kExact ? exp_exact(-v) : exp2_fast(v * -kLog2e)));
 }
 
 }  // namespace rgk

@@ -47,7 +47,7 @@ template <bool kExact>
 __device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
   Pair e;
   if constexpr (kExact) {
-    e = pair(exp_exact(-fabsf(v0)), exp_exact(-fabsf(v1)));
+    e = exp_exact(-fabsf(v0), -fabsf(v1));
   } else {
     e = exp2_pair(mul2(pair(fabsf(v0), fabsf(v1)), pair(-kLog2e, -kLog2e)));
   }
@@ -388,7 +388,7 @@ selective_scan_kernel(const SelectiveArgs p) {
             widen4(raw(stage, 2) + t * kChan + 4 * q, vz);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-              const float2 gate = silu_fast(vz[i], vz[i + 1]);
+              const float2 gate = silu_fast<sizeof(T) == 4>(vz[i], vz[i + 1]);
               out[i] *= gate.x; out[i + 1] *= gate.y;
             }
           }
@@ -708,7 +708,7 @@ selective_step_kernel(const SelectiveArgs p) {
     for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (l == 0 && in) {
       float out = fmaf(d, xr, sum);
-      if (p.z != nullptr) out *= silu_fast(static_cast<float>(z[r]), 0.0f).x;
+      if (p.z != nullptr) out *= silu_fast<sizeof(T) == 4>(static_cast<float>(z[r]));
       static_cast<T*>(p.y)[b * p.E + e] = static_cast<T>(out);
     }
   }
@@ -806,7 +806,7 @@ selective_steps_kernel(const SelectiveArgs p, int per) {
     for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (l == 0 && in) {
       float out = fmaf(d, x, sum);
-      if (gated) out *= silu_fast(static_cast<float>(v.z), 0.0f).x;
+      if (gated) out *= silu_fast<sizeof(T) == 4>(static_cast<float>(v.z));
       *y = static_cast<T>(out);
     }
     y += p.E;
