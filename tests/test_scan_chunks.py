@@ -45,3 +45,57 @@ def test_chunks_where_only_a_part_of_the_grid_finds_a_place():
     rg.check_status()
     for g, w in zip(got, (held, *want)):
       assert all(torch.equal(p, q) for p, q in zip(g, w))
+
+
+# More blocks of channels (128 a CTA at most, two CTAs an SM) than CTAs, and 512 steps or more: time is cut, whichever
+# shape the number of states has.  Rows aligned to copies of 16 bytes, but for the last ones.
+CHUNKED = [
+    # b, t, e, n, groups, doc, options
+    (8, 520, 5120, 16, 1, 90, {}),
+    (8, 641, 5120, 16, 1, 0, dict(state=False, z=False)),
+    (8, 520, 5120, 3, 1, 200, {}),
+    (8, 520, 5120, 8, 2, 90, {}),
+    (8, 520, 5120, 32, 1, 90, {}),
+    (4, 530, 5120, 64, 1, 300, {}),
+    (4, 520, 2560, 128, 1, 90, {}),
+    (2, 513, 2560, 256, 1, 0, {}),
+    (8, 515, 5130, 16, 2, 90, dict(part=True)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,t,e,n,groups,doc,options", CHUNKED)
+def test_scan_in_chunks_of_time(b, t, e, n, groups, doc, options, dtype):
+  """Against the definition, the state passed on beside the one that was given and over it."""
+  import recurrentgemma_b200 as rg
+  from tests.test_state_space import scan_case, scan_definition, within
+  case = scan_case(t + n, b, t, e, n, dtype, groups, doc, **options)
+  want, held, bound, bound_state = scan_definition(**case)
+  y, state = rg.selective_scan(**case)
+  within(y, want, bound, dtype)
+  within(state, held, bound_state, torch.float32)
+  given = torch.zeros(b, e, n, device="cuda") if case["state"] is None else case["state"].clone()
+  again, back = rg.selective_scan(**{**case, "state": given}, inplace=True)
+  assert back is given and torch.equal(back, state) and torch.equal(again, y)
+  rg.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("taps,doc,half", [(4, 0, True), (4, 30, False), (3, 0, False), (2, 500, True)])
+def test_convolution_of_a_prefill_batch(taps, doc, half, dtype):
+  """Large enough for a thread's longest run of rows, in packs: 16 a thread, which 12 M elements and more take."""
+  import recurrentgemma_b200 as rg
+  from tests.test_state_space import conv_case, conv_definition, within
+  b, t, e = 6, 803, 2560
+  case = conv_case(taps + doc, b, t, e, taps, dtype, doc)
+  if half:                                           # (one half of a projection's output)
+    case["x"] = torch.cat([case["x"], case["x"]], -1)[..., :e]
+  want, held, bound = conv_definition(**case)
+  y, state = rg.causal_conv(**case)
+  within(y, want, bound, dtype)
+  assert torch.equal(state.double(), held)
+  given = case["state"].clone()
+  again, back = rg.causal_conv(**{**case, "state": given}, inplace=True)
+  assert back is given and torch.equal(back, state) and torch.equal(again, y)
