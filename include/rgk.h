@@ -491,6 +491,7 @@ RGK_API int rgk_geglu_bias(const void* up, const void* bias, int64_t M, int64_t 
  *   group g = e / (E / groups) and its N states (1 to 256):
  *     h_t[n] = exp(D_t a[e,n]) h_{t-1}[n] + D_t x_t b_t[g,n]  (a document start drops h_{t-1}),
  *     y_t = (sum_n h_t[n] c_t[g,n] + d[e] x_t) silu(z_t).
+ *   (Where x_t or D_t is infinite, y may be NaN instead of infinite; the states are as the formula has them.)
  *   x, dt, z (or NULL) [B,T,E], b, c [B,T,groups,N]; a [E,N], d [E] or NULL, dt_bias [E] or NULL and the
  *   states [B,E,N] are float32.  state_in NULL: zeros; state_out: NULL, or it may be state_in.  T may be 0.
  *   workspace: NULL, or rgk_selective_scan_workspace_bytes() of scratch (4-byte aligned, of any content, of no other

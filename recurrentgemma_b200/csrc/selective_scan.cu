@@ -353,6 +353,10 @@ selective_scan_kernel(const SelectiveArgs p) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) steps(buf)[t * kChan + i * kQuads + q] = make_float2(step[i], step[i] * vx[i]);
         }
+        if (tile == 0 && chunk == 0 && p.state_in == nullptr && row0 == 0) {     // as at a start, without a state
+#pragma unroll
+          for (int i = 0; i < 4; ++i) steps(buf)[i * kQuads + q].x = 0.0f;
+        }
       };
       // its outputs
       auto finish = [&](int tile) {
@@ -488,7 +492,9 @@ selective_scan_kernel(const SelectiveArgs p) {
 #pragma unroll
               for (int c = 0; c < C; ++c) {
                 const float2 step = s_step[t * kChan + owner + c * Sh::kOwners];
-                const Pair step2 = pair(step.x, step.x), put2 = pair(step.y, step.y);
+                // (at a start the factor is 1: one that has overflowed would not be dropped by what it multiplies)
+                const float by = decltype(with_starts)::value && ((starts >> t) & 1u) ? 0.0f : step.x;
+                const Pair step2 = pair(by, by), put2 = pair(step.y, step.y);
                 Pair both = 0;
 #pragma unroll
                 for (int s = 0; s < S / 2; ++s) {
@@ -618,10 +624,11 @@ selective_step_kernel(const SelectiveArgs p) {
   float4 h[kRows][Q];
   Raw vb[kRows][Q], vc[kRows][Q];
   T x[kRows], dt[kRows], z[kRows];
+  bool fresh[kRows];                                             // nothing of what was held counts
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t b = min(b0 + r, p.B - 1);
-    const bool fresh = p.state_in == nullptr || (p.pos != nullptr && pos_is_zero(p.pos, p.pos64, b));
+    fresh[r] = p.state_in == nullptr || (p.pos != nullptr && pos_is_zero(p.pos, p.pos64, b));
     const float* from = p.state_in + (b * p.E + e) * p.N;
     const T* rb = static_cast<const T*>(p.b) + b * p.b_batch + (int64_t)g * p.N;
     const T* rc = static_cast<const T*>(p.c) + b * p.c_batch + (int64_t)g * p.N;
@@ -632,7 +639,7 @@ selective_step_kernel(const SelectiveArgs p) {
       vb[r][k] = vc[r][k] = Raw{};
       if (kVec) {
         if (n < p.N) {
-          if (!fresh) h[r][k] = *reinterpret_cast<const float4*>(from + n);
+          if (!fresh[r]) h[r][k] = *reinterpret_cast<const float4*>(from + n);
           vb[r][k] = *reinterpret_cast<const Raw*>(rb + n);
           vc[r][k] = *reinterpret_cast<const Raw*>(rc + n);
         }
@@ -640,7 +647,7 @@ selective_step_kernel(const SelectiveArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (n + i < p.N) {
-            if (!fresh) (&h[r][k].x)[i] = from[n + i];
+            if (!fresh[r]) (&h[r][k].x)[i] = from[n + i];
             reinterpret_cast<T*>(&vb[r][k])[i] = rb[n + i];
             reinterpret_cast<T*>(&vc[r][k])[i] = rc[n + i];
           }
@@ -675,7 +682,7 @@ selective_step_kernel(const SelectiveArgs p) {
     const float xr = static_cast<float>(x[r]);
     float now = static_cast<float>(dt[r]) + bias;
     if (p.softplus) now = softplus_step<sizeof(T) == 4>(now);
-    const float put = now * xr;
+    const float put = now * xr, by = fresh[r] ? 0.0f : now;       // (a factor that has overflowed multiplies nothing)
     float sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
@@ -686,7 +693,7 @@ selective_step_kernel(const SelectiveArgs p) {
       widen4(h[r][k], fh);
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        const float2 decay = decays<kExact>(now, a2[4 * k + i], a2[4 * k + i + 1]);
+        const float2 decay = decays<kExact>(by, a2[4 * k + i], a2[4 * k + i + 1]);
         fh[i] = fmaf(decay.x, fh[i], put * fb[i]);
         fh[i + 1] = fmaf(decay.y, fh[i + 1], put * fb[i + 1]);
         sum = fmaf(fh[i], fc[i], sum);
@@ -778,7 +785,8 @@ selective_steps_kernel(const SelectiveArgs p, int per) {
     if (r + 1 < rows) next = inputs();
     asm volatile("cp.async.wait_group %0;" :: "n"(kDepth - 1) : "memory");
     float h[4] = {0.0f, 0.0f, 0.0f, 0.0f}, fb[4], fc[4];
-    if (held && !(p.pos != nullptr && pos_is_zero(p.pos, p.pos64, b0 + r))) {
+    const bool fresh = !held || (p.pos != nullptr && pos_is_zero(p.pos, p.pos64, b0 + r));
+    if (!fresh) {
       const float4 was = ring[r % kDepth][threadIdx.x];
       h[0] = was.x; h[1] = was.y; h[2] = was.z; h[3] = was.w;
     }
@@ -787,11 +795,11 @@ selective_steps_kernel(const SelectiveArgs p, int per) {
     const float x = static_cast<float>(v.x);
     float now = static_cast<float>(v.dt) + bias;
     if (p.softplus) now = softplus_step<sizeof(T) == 4>(now);
-    const float put = now * x;
+    const float put = now * x, by = fresh ? 0.0f : now;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
-      const float2 decay = decays<kExact>(now, a2[i], a2[i + 1]);
+      const float2 decay = decays<kExact>(by, a2[i], a2[i + 1]);
       h[i] = fmaf(decay.x, h[i], put * fb[i]);
       h[i + 1] = fmaf(decay.y, h[i + 1], put * fb[i + 1]);
       sum = fmaf(h[i], fc[i], sum);

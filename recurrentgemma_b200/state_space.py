@@ -108,7 +108,8 @@ def selective_scan(
   d [E] and dt_bias [E] float32 (a is the decay rate itself, negative in trained layers).  `state` [B,E,N]
   float32 is h in front of the first token (None: zeros); a decode step is a call with one token.  A document
   start (segment_pos == 0) drops the state in front of it.  `inplace` overwrites `state` and returns it.
-  x, dt, z, b and c may be strided over batch and time.
+  x, dt, z, b and c may be strided over batch and time.  Where x or a step is infinite, y may be NaN instead of
+  infinite; the states are as the formula has them.
   """
   done = _lib.host().selective_scan(x, dt, a, b, c, d, z, dt_bias, segment_pos, state, softplus, return_state,
                                     inplace)
