@@ -375,7 +375,8 @@ struct SampleArgs {
   float top_p_value, min_p_value;
   int bits;                              // of a weight's fraction
   int* out;
+  struct Groups { int lanes, per_warp, groups, most_k; } coarse, fine;   // of a row's lanes (set by the launcher)
 };
-cudaError_t launch_sample(const SampleArgs& p, int dtype, cudaStream_t s);
+cudaError_t launch_sample(SampleArgs p, int dtype, cudaStream_t s);
 
 }  // namespace rgk

@@ -15,13 +15,14 @@
 // that it ends in hold at most 2048 tokens, those are brought together in index order, and one CTA sorts them and does
 // the rest; otherwise the bin's own tokens are, which gives the last token kept, and the draw runs over the row.  A bin
 // with more tokens than that (ties, huge temperatures) is cut into 2048 ranges of keys, and again if need be; a single
-// key is cut by counting.  For top-k up to 128 there is no histogram: the k-th largest of the maxima of 128 parts of the
-// row bounds what can be among the first k.
+// key is cut by counting.  For top-k up to 128 there is mostly no histogram: the k-th largest of the maxima of 128 parts of
+// the row, or more, bounds what can be among the first k (unless more than 2048 tokens are as large as that).
 //
 // Bound: 2 or 4 bytes a token from HBM, and for whole rows and top-p without top-k the 64-bit exponential of every token
 // within 31 temperatures of the maximum (11 double-precision operations, 2 cycles of a scheduler each).
 #include <float.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "rgk_common.cuh"
@@ -42,7 +43,7 @@ constexpr int kMostParts = 8;
 constexpr float kRange = 32.0f;                                   // temperatures below the maximum: W = 0 from 31.2 on
 constexpr int kTable = 64;
 constexpr int kStretches = 16;
-constexpr int kGroups = 128;                                      // of a row's threads
+constexpr int kMostK = 128, kMostGroups = 320;                    // of top-k by groups of a row's lanes
 
 // The order of the floats as an order of integers (-0 counts as 0, NaN below everything).
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -142,7 +143,8 @@ struct Shared {
   float best[kMostParts];
   int best_at[kMostParts];
   unsigned key_lo[kMostParts], key_hi[kMostParts];
-  float groups[kGroups], least;                                   // maxima of parts of the row, and one of them
+  alignas(16) float groups[kMostGroups + 4];                      // maxima of parts of the row
+  float least;                                                    // one of them
   Found found;
   unsigned length;                                                // of the list
   unsigned mine, place;                                           // of it in this CTA: how many, and from where on
@@ -216,6 +218,12 @@ template <typename T> struct Row {
   }
   template <typename F> __device__ __forceinline__ void each(F&& fn) const { each(fn, [](int) {}); }
 };
+
+// How many packs a warp takes of a row.
+__host__ __device__ __forceinline__ int run_of(int packs, int parts) {
+  const int run = (packs + parts * kWarps - 1) / (parts * kWarps);
+  return run > 64 ? (run + 32 * kAhead - 1) / (32 * kAhead) * (32 * kAhead) : run;       // (whole rounds of `each`)
+}
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
@@ -623,6 +631,7 @@ __device__ bool prefix(const Row<T>& row, Shared& sh, const Weights& weight, Bin
 }
 
 template <typename V> __device__ __forceinline__ V setting(const V* p, V value, int64_t m) { return p != nullptr ? p[m] : value; }
+__device__ __forceinline__ int top_k_of(const SampleArgs& p, int64_t m) { return setting(p.top_k, p.top_k_value, m); }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -638,8 +647,7 @@ sample_kernel(const SampleArgs p, int parts) {
   row.parts = parts;
   row.rank = (int)(blockIdx.x - m * parts);
   const int packs = (row.head + row.V + kPer - 1) / kPer;
-  int run = (packs + parts * kWarps - 1) / (parts * kWarps);
-  if (run > 64) run = (run + 32 * kAhead - 1) / (32 * kAhead) * (32 * kAhead);        // (whole rounds of `each`)
+  const int run = run_of(packs, parts);
   row.begin = min(packs, (row.rank * kWarps + warp) * run);
   row.end = min(packs, row.begin + run);
   if (parts > 1) cluster_arrive();                                // "this CTA runs"
@@ -657,7 +665,9 @@ sample_kernel(const SampleArgs p, int parts) {
   auto better = [&](float ob, int oa) {
     if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
   };
-  const int group = kThreads * parts / kGroups;                   // lanes: 4, 8, 16 or 32
+  // (In a row that begins inside of a pack a group may be without a token, or not be asked: a bound it is all the same.)
+  const bool fine = top_k_of(p, m) > p.coarse.most_k;
+  const int group = fine ? p.fine.lanes : p.coarse.lanes;
   float of_group = best;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -674,8 +684,13 @@ sample_kernel(const SampleArgs p, int parts) {
     peer(&sh, tid)->best[row.rank] = best;
     peer(&sh, tid)->best_at[row.rank] = at;
   }
-  if (lane % group == 0) {
-    for (int r = 0; r < parts; ++r) peer(&sh, r)->groups[(row.rank * kThreads + tid) / group] = of_group;
+  {
+    const int per_warp = fine ? p.fine.per_warp : p.coarse.per_warp, groups = fine ? p.fine.groups : p.coarse.groups;
+    const int at_group = (row.rank * kWarps + warp) * per_warp + lane / group;
+    if (lane % group == 0 && lane / group < per_warp && at_group < groups) {
+      for (int r = 0; r < parts; ++r) peer(&sh, r)->groups[at_group] = of_group;
+    }
+    if (tid < 4) sh.groups[groups + tid] = -INFINITY;             // (read in fours)
   }
   row.sync();
   for (int r = 0; r < parts; ++r) better(sh.best[r], sh.best_at[r]);
@@ -688,7 +703,7 @@ sample_kernel(const SampleArgs p, int parts) {
   best += 0.0f;
   const Weights weight{1.4426950408889634 / (double)temperature, (double)best, p.bits, sh.table};
   Settings set;
-  set.top_k = setting(p.top_k, p.top_k_value, m);
+  set.top_k = top_k_of(p, m);
   if (set.top_k < 0 || set.top_k >= row.V) set.top_k = 0;
   set.top_p = setting(p.top_p, p.top_p_value, m);
   const double min_p = (double)setting(p.min_p, p.min_p_value, m);
@@ -711,15 +726,21 @@ sample_kernel(const SampleArgs p, int parts) {
   int n = 0;
   u64 wanted = 0;
   bool listed = false;
-  if (set.top_k > 0 && set.top_k <= kGroups) {
+  if (set.top_k > 0 && set.top_k <= kMostK) {
     // The k-th largest of the groups' maxima: k tokens are at least that, so the first k of all are among those that
-    // are.  Mostly they are few (some 60 for k = 50, 600 for k = 128).
-    if (tid < kGroups) {
+    // are.  Mostly they are few (some 60 for k = 50, 200 for k = 100 or 128).  Fewer than k groups are there only in rows of
+    // fewer than 512 tokens: all of those.
+    const int groups = fine ? p.fine.groups : p.coarse.groups;
+    if (tid < groups) {
       const float mine = sh.groups[tid];
       int place = 0;
-#pragma unroll 8
-      for (int i = 0; i < kGroups; ++i) place += sh.groups[i] > mine || (sh.groups[i] == mine && i < tid);
-      if (place == set.top_k - 1) sh.least = mine;
+#pragma unroll 4
+      for (int i = 0; i < groups; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(sh.groups + i);
+        place += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
+                 (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
+      }
+      if (place == min(set.top_k, groups) - 1) sh.least = set.top_k <= groups ? mine : -INFINITY;
     }
     __syncthreads();
     const float least = sh.least;
@@ -751,7 +772,26 @@ sample_kernel(const SampleArgs p, int parts) {
 
 }  // namespace
 
-cudaError_t launch_sample(const SampleArgs& p, int dtype, cudaStream_t s) {
+// Groups of neighbouring lanes of a row, for top-k: a quarter more than k of them that have tokens, if there are as many
+// such lanes.  A warp's run is rounded up, so that the last warps may be without: counted are the whole runs and what
+// is left of a row, one run at most (of 128 groups by threads alone 65 have tokens of 33000, 99 of 151936).  One row of 151936
+// tokens takes 14 us for k = 50 with coarse groups, and for k = 100 16 us with fine ones; where there are fewer groups than k, a
+// histogram has to find the k-th: 31 us.
+static void group_lanes(SampleArgs* p, int parts) {
+  const int packs = (int)((p->V + kPer - 1) / kPer), run = run_of(packs, parts);
+  auto groups_by = [&](int lanes) {
+    const int per_warp = (std::min(run, 32) + lanes - 1) / lanes;
+    const int groups = packs / run * per_warp + (std::min(packs % run, 32) + lanes - 1) / lanes;
+    return SampleArgs::Groups{lanes, per_warp, groups, groups * 4 / 5};
+  };
+  int lanes = kThreads * parts / kMostK;                          // 4, 8, 16 or 32: 128 groups, where all have tokens
+  p->coarse = groups_by(lanes);
+  // (never more than kMostGroups: with twice the lanes there are fewer than 5/4 of kMostK)
+  while (lanes > 1 && groups_by(lanes).most_k < kMostK) lanes /= 2;
+  p->fine = groups_by(lanes);
+}
+
+cudaError_t launch_sample(SampleArgs p, int dtype, cudaStream_t s) {
   if (p.M == 0) return cudaSuccess;
   static PerDeviceOnce once;
   int sms = 0;
@@ -766,6 +806,7 @@ cudaError_t launch_sample(const SampleArgs& p, int dtype, cudaStream_t s) {
   // 567 us, on 64 rows 209 / 125 / 110 / 149, on 16 rows 208 / 125 / 79 / 74, on one row 199 / 117 / 72 / 52.
   int parts = kMostParts;
   while (parts > 1 && (p.V < parts * 4096 || p.M * parts > 2 * sms)) parts /= 2;
+  group_lanes(&p, parts);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)parts;
