@@ -706,6 +706,7 @@ sample_kernel(const SampleArgs p, int parts) {
   set.top_k = top_k_of(p, m);
   if (set.top_k < 0 || set.top_k >= row.V) set.top_k = 0;
   set.top_p = setting(p.top_p, p.top_p_value, m);
+  if (set.top_p < 0.0f) set.top_p = 0.0f;
   const double min_p = (double)setting(p.min_p, p.min_p_value, m);
   set.least = min_p > 0.0 ? (u64)ceil(fmin(min_p, 1.0) * (double)weight.unit()) : 0ull;
   set.uniform = p.uniforms[m];
@@ -751,7 +752,7 @@ sample_kernel(const SampleArgs p, int parts) {
     listed = prefix<true, false>(row, sh, weight, bins, best, cut, -1.0, (u64)set.top_k, &cut, &n, &wanted);
   if (!listed && set.top_p < 1.0f) {
     set.top_k = 0;                                                // (in the cut by now)
-    const double share = fmax((double)set.top_p, 0.0);
+    const double share = (double)set.top_p;
     listed = cut.last < 0 ? prefix<false, false>(row, sh, weight, bins, best, cut, share, 0, &cut, &n, &wanted)
                           : prefix<false, true>(row, sh, weight, bins, best, cut, share, 0, &cut, &n, &wanted);
   }

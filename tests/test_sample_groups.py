@@ -41,3 +41,23 @@ def test_parts_of_a_row_without_a_token(v):
     for u in (0.0, 0.4, 1.0 - 2.0 ** -24):
       uniforms = torch.full((6,), u, device="cuda")
       assert torch.equal(rg.sample(logits, uniforms, top_k=k), definition(logits, uniforms, top_k=k)), (k, u)
+
+
+@pytest.mark.gpu
+def test_settings_of_rows_below_their_range():
+  """Only numbers are refused on the host: in a tensor a top_p below 0 keeps one token, a min_p below 0 all, one above 1 the
+  largest, a temperature below 0 is greedy and a top_k below 0 keeps all."""
+  import recurrentgemma_b200 as rg
+  logits, u, _ = rows(7, 6, 5000, torch.float32)
+  logits[3] = logits[3].round()                      # (ties at the top)
+  logits[4, 7], logits[4, 1900] = math.inf, math.inf
+  row = lambda v: torch.full((6,), v, device="cuda")                             # noqa: E731
+  best = definition(logits, u, temperature=0.0)
+  for k in (0, 50, 3000):
+    assert torch.equal(rg.sample(logits, u, top_k=k, top_p=row(-0.5)), best)
+    assert torch.equal(rg.sample(logits, u, top_k=k, top_p=row(-math.inf)), best)
+  assert torch.equal(rg.sample(logits, u, temperature=row(-1.0)), best)
+  every = rg.sample(logits, u)
+  assert torch.equal(rg.sample(logits, u, min_p=row(-2.0)), every)
+  assert torch.equal(rg.sample(logits, u, top_k=torch.full((6,), -9, dtype=torch.int32, device="cuda")), every)
+  assert torch.equal(rg.sample(logits, u, min_p=row(7.0)), rg.sample(logits, u, min_p=1.0))
