@@ -179,14 +179,14 @@ cudaError_t launch_rows(ConvArgs p, cudaStream_t s) {
 }
 
 template <typename T, int kPer>
-cudaError_t launch_pack(const ConvArgs& p, cudaStream_t s) {
+cudaError_t launch_pack(const ConvArgs& p, int sms, cudaStream_t s) {
   // Many rows a thread where that still fills the device (8 x 4096 x 5120 in bfloat16 with 8 / 12 / 16 / 24 rows:
   // 139 / 130 / 124 / 127 us; 3 x 1237 x 2565 in float32, a channel a thread: 31 / 29 / 41 / 46), four where it
   // does not.  (From W-1 rows on a sequence's first chunk is the only one that reads the state, so that it may be
   // written in place.)
   constexpr int kMany = kPer > 1 ? 16 : 12;
   if (p.T <= 1) return launch_rows<T, kPer, 1>(p, s);
-  if (p.B * p.T * (p.E / kPer) >= kMany * (int64_t)148 * 1024) return launch_rows<T, kPer, kMany>(p, s);
+  if (p.B * p.T * (p.E / kPer) >= kMany * (int64_t)sms * 1024) return launch_rows<T, kPer, kMany>(p, s);
   return launch_rows<T, kPer, 4>(p, s);
 }
 
@@ -194,12 +194,16 @@ cudaError_t launch_pack(const ConvArgs& p, cudaStream_t s) {
 
 cudaError_t launch_causal_conv(const ConvArgs& p, int dtype, cudaStream_t s) {
   if (p.B == 0 || p.E == 0) return cudaSuccess;
+  static PerDeviceOnce once;
+  int sms = 0;
+  const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
+  if (e != cudaSuccess) return e;
   const int per = dtype == 1 ? 4 : 2;
   auto fits = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 7u) == 0; };
   const bool packs = p.E % per == 0 && p.x_token % per == 0 && p.x_batch % per == 0 && fits(p.x) && fits(p.w) &&
                      fits(p.bias) && fits(p.state_in) && fits(p.state_out) && fits(p.y);
-  if (dtype == 1) return packs ? launch_pack<__nv_bfloat16, 4>(p, s) : launch_pack<__nv_bfloat16, 1>(p, s);
-  return packs ? launch_pack<float, 2>(p, s) : launch_pack<float, 1>(p, s);
+  if (dtype == 1) return packs ? launch_pack<__nv_bfloat16, 4>(p, sms, s) : launch_pack<__nv_bfloat16, 1>(p, sms, s);
+  return packs ? launch_pack<float, 2>(p, sms, s) : launch_pack<float, 1>(p, sms, s);
 }
 
 }  // namespace rgk

@@ -822,7 +822,7 @@ selective_steps_kernel(const SelectiveArgs p, int per) {
 }
 
 template <typename T, int S, int L>
-cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
+cudaError_t launch_step(const SelectiveArgs& p, int sms, cudaStream_t s) {
   auto fits = [&](const void* q, int64_t batch, int size) {
     return (reinterpret_cast<uintptr_t>(q) | (uint64_t)(batch * size)) % (4 * size) == 0;
   };
@@ -831,10 +831,6 @@ cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
   const unsigned across = (unsigned)((p.E + 256 / L - 1) / (256 / L));
   if constexpr (S == 4) {
     if (vec) {
-      static PerDeviceOnce once;
-      int sms = 0;
-      const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
-      if (e != cudaSuccess) return e;
       // eight sequences a thread and more where four CTAs an SM have that many
       const int64_t down = max((int64_t)1, (int64_t)4 * sms / across), per = (p.B + down - 1) / down;
       if (per >= 8)
@@ -845,7 +841,7 @@ cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
     }
   }
   // four sequences a thread where they still give every SM its threads
-  const bool many = across * p.B >= 4 * 8 * 148;
+  const bool many = across * p.B >= 4 * 8 * (int64_t)sms;
   const dim3 grid(across, (unsigned)(many ? (p.B + 3) / 4 : p.B));
   if constexpr (S != 4) {
     if (vec && many) selective_step_kernel<T, S, L, 4, true><<<grid, 256, 0, s>>>(p);
@@ -857,14 +853,14 @@ cudaError_t launch_step(const SelectiveArgs& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 template <typename T>
-cudaError_t launch_step_states(const SelectiveArgs& p, cudaStream_t s) {
-  if (p.N <= 4) return launch_step<T, 4, 1>(p, s);
-  if (p.N <= 8) return launch_step<T, 4, 2>(p, s);
-  if (p.N <= 16) return launch_step<T, 4, 4>(p, s);
-  if (p.N <= 32) return launch_step<T, 4, 8>(p, s);
-  if (p.N <= 64) return launch_step<T, 4, 16>(p, s);
-  if (p.N <= 128) return launch_step<T, 4, 32>(p, s);
-  return launch_step<T, 8, 32>(p, s);
+cudaError_t launch_step_states(const SelectiveArgs& p, int sms, cudaStream_t s) {
+  if (p.N <= 4) return launch_step<T, 4, 1>(p, sms, s);
+  if (p.N <= 8) return launch_step<T, 4, 2>(p, sms, s);
+  if (p.N <= 16) return launch_step<T, 4, 4>(p, sms, s);
+  if (p.N <= 32) return launch_step<T, 4, 8>(p, sms, s);
+  if (p.N <= 64) return launch_step<T, 4, 16>(p, sms, s);
+  if (p.N <= 128) return launch_step<T, 4, 32>(p, sms, s);
+  return launch_step<T, 8, 32>(p, sms, s);
 }
 
 // There is a choice of shapes: few states a thread keep a step short where channels are few, many states and two channels
@@ -891,11 +887,7 @@ int quickest(const Choice (&of)[kCount], const SelectiveArgs& p, int sms) {
 // 64 states 120 / 443 / 875 / 1734, 104 / 285 / 554 / 1091, 114 / 236 / 440 / 870;   128 states 168 / 627 / 1237,
 // 191 / 497 / 989.
 template <typename T>
-cudaError_t launch_states(const SelectiveArgs& p, cudaStream_t s) {
-  static PerDeviceOnce once;
-  int sms = 0;
-  const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
-  if (e != cudaSuccess) return e;
+cudaError_t launch_states(const SelectiveArgs& p, int sms, cudaStream_t s) {
   if (p.N <= 4) return launch<T, 4, 1, 1, 16>(p, s);
   if (p.N <= 8) {
     return quickest({{57, 64}, {95, 128}}, p, sms) == 0 ? launch<T, 4, 1, 2, 16>(p, s) : launch<T, 4, 2, 2, 16>(p, s);
@@ -942,14 +934,18 @@ size_t selective_workspace_bytes() { return (1 + kMostBlocks) * sizeof(int); }
 cudaError_t launch_selective_scan(SelectiveArgs p, int dtype, cudaStream_t s) {
   if (p.B == 0 || p.E == 0) return cudaSuccess;
   const int size = dtype == 1 ? 2 : 4;
+  static PerDeviceOnce once;
+  int sms = 0;
+  const cudaError_t e = once.run([] { return cudaSuccess; }, &sms);
+  if (e != cudaSuccess) return e;
   p.per_group = (int)(p.E / p.groups);
-  if (p.T == 1) return dtype == 1 ? launch_step_states<__nv_bfloat16>(p, s) : launch_step_states<float>(p, s);
+  if (p.T == 1) return dtype == 1 ? launch_step_states<__nv_bfloat16>(p, sms, s) : launch_step_states<float>(p, sms, s);
   p.copy_x = min(copy_bytes(p.x, p.x_batch, p.x_token, p.per_group, size),
                  copy_bytes(p.dt, p.dt_batch, p.dt_token, p.per_group, size));
   if (p.z != nullptr) p.copy_x = min(p.copy_x, copy_bytes(p.z, p.z_batch, p.z_token, p.per_group, size));
   p.copy_n = min(copy_bytes(p.b, p.b_batch, p.b_token, p.N, size), copy_bytes(p.c, p.c_batch, p.c_token, p.N, size));
   p.store4 = p.per_group % 4 == 0 && p.E % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % (4 * size) == 0;
-  return dtype == 1 ? launch_states<__nv_bfloat16>(p, s) : launch_states<float>(p, s);
+  return dtype == 1 ? launch_states<__nv_bfloat16>(p, sms, s) : launch_states<float>(p, sms, s);
 }
 
 }  // namespace rgk

@@ -99,3 +99,11 @@ def test_convolution_of_a_prefill_batch(taps, doc, half, dtype):
   given = case["state"].clone()
   again, back = rg.causal_conv(**{**case, "state": given}, inplace=True)
   assert back is given and torch.equal(back, state) and torch.equal(again, y)
+
+
+@pytest.mark.parametrize("name", ["causal_conv.cu", "selective_scan.cu", "sample.cu"])
+def test_launchers_ask_for_the_number_of_sms(name):
+  """No kernel is chosen by the number of SMs of one device."""
+  with open(os.path.join(CSRC, name)) as f:
+    text = re.sub(r"//[^\n]*", "", f.read())
+  assert not re.search(r"\b148\b", text)
