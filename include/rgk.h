@@ -507,6 +507,7 @@ RGK_API int rgk_geglu_bias(const void* up, const void* bias, int64_t M, int64_t 
  *   Every setting is an array of M on the device, or NULL: the value beside it for all rows.
  * ---------------------------------------------------------------------------------------------- */
 enum { RGK_CONV_ACT_NONE = 0, RGK_CONV_ACT_SILU = 1 };
+enum { RGK_SCAN_CHUNKS_FROM = 512 };        /* shorter selective scans make no use of a workspace */
 RGK_API int rgk_causal_conv(const void* x, int64_t x_batch, int64_t x_token, const void* segment_pos,
                             int pos_dtype, const void* w, const void* bias, const void* state_in, int64_t B,
                             int64_t T, int64_t E, int W, int act, int dtype, void* y, void* state_out,

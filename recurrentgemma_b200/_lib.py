@@ -25,6 +25,7 @@ RGK_F32, RGK_BF16 = 0, 1
 RGK_I32, RGK_I64 = 0, 1
 ACT_NONE, ACT_GELU_TANH, ACT_GEGLU = 0, 1, 2
 CONV_ACT_NONE, CONV_ACT_SILU = 0, 1
+SCAN_CHUNKS_FROM = 512         # RGK_SCAN_CHUNKS_FROM
 GATES_AUTO, GATES_SIMT, GATES_TCGEN05, GATES_FUSED, GATES_FUSED_EXACT = 0, 1, 2, 3, 4
 
 _vp, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t

@@ -764,6 +764,7 @@ int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int p
   return RGK_OK;
 }
 
+static_assert(rgk::kScanChunksFrom == RGK_SCAN_CHUNKS_FROM, "as the callers have it");
 size_t rgk_selective_scan_workspace_bytes(void) { return rgk::selective_workspace_bytes(); }
 
 int rgk_sample(const void* logits, int64_t M, int64_t V, int64_t row_stride, int dtype, const float* uniforms,

@@ -829,7 +829,7 @@ PyObject* selective_scan(PyObject* const* args, Py_ssize_t n) {
   // a long call's scratch is its own (captured calls may be replayed side by side); timeouts show up in check_status
   Workspace ws;
   at::Tensor scratch;
-  if (T >= 512) {
+  if (T >= RGK_SCAN_CHUNKS_FROM) {
     if (!workspace(*x, s, 4, &ws)) return nullptr;
     scratch = empty({(int64_t)g_lib.selective_scan_workspace_bytes()}, at::kByte, x->device());
   }

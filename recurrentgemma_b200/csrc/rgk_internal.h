@@ -358,6 +358,7 @@ struct SelectiveArgs {
   int64_t blocks, chunk, chunks;         // of channels; of time: length and number
   int* done;                             // chunks that a block has done
 };
+constexpr int kScanChunksFrom = 512;     // time steps: shorter calls make no use of the scratch
 size_t selective_workspace_bytes();
 cudaError_t launch_selective_scan(SelectiveArgs p, int dtype, cudaStream_t s);
 

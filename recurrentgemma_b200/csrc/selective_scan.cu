@@ -560,7 +560,7 @@ cudaError_t launch_kernel(SelectiveArgs p, cudaStream_t s) {
   if (p.blocks >= ((int64_t)1 << 31)) return cudaErrorInvalidValue;
   int64_t grid = p.blocks;
   // Chunks of time drawn by a ticket.
-  if (p.ticket != nullptr && p.state_out != nullptr && p.T >= 512) {
+  if (p.ticket != nullptr && p.state_out != nullptr && p.T >= kScanChunksFrom) {
     int per_sm = 0;
     if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, selective_scan_kernel<T, Sh, kAligned>, 2 * kTeam,
                                                            Sh::kBytes)) != cudaSuccess) return e;

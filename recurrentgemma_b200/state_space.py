@@ -148,10 +148,11 @@ def _selective_scan(x, dt, a, b, c, d, z, dt_bias, segment_pos, state, softplus,
       *(_lib.ptr(t) for t in params), int(softplus))
   with torch.cuda.device(dev):
     lib = _lib.load()
-    # (scratch of this call alone: captured calls may be replayed side by side)
-    ws = torch.empty(lib.rgk_selective_scan_workspace_bytes(), dtype=torch.uint8, device=dev)
+    # (a long call has scratch of its own: captured calls may be replayed side by side)
+    ws = (torch.empty(lib.rgk_selective_scan_workspace_bytes(), dtype=torch.uint8, device=dev)
+          if l >= _lib.SCAN_CHUNKS_FROM else None)
     _lib.check(lib.rgk_selective_scan(
         ctypes.byref(p), _lib.ptr(pos), 0 if pos is None else _lib.pos_code(pos), _lib.ptr(sc), bs, l, e,
-        groups, n, code, y.data_ptr(), new_state.data_ptr(), ws.data_ptr(), ws.numel(), _lib.status_ptr(dev),
-        _lib.stream_ptr(dev)))
+        groups, n, code, y.data_ptr(), new_state.data_ptr(), _lib.ptr(ws), 0 if ws is None else ws.numel(),
+        _lib.status_ptr(dev), _lib.stream_ptr(dev)))
   return y, (new_state if return_state else None)

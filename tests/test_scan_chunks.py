@@ -107,3 +107,32 @@ def test_launchers_ask_for_the_number_of_sms(name):
   with open(os.path.join(CSRC, name)) as f:
     text = re.sub(r"//[^\n]*", "", f.read())
   assert not re.search(r"\b148\b", text)
+
+
+def test_length_from_which_scratch_is_used():
+  """The one of the header, on both sides."""
+  from recurrentgemma_b200 import _lib
+  root = os.path.dirname(os.path.dirname(os.path.dirname(CSRC + "/")))
+  with open(os.path.join(root, "include", "rgk.h")) as f:
+    assert int(re.search(r"RGK_SCAN_CHUNKS_FROM = (\d+)", f.read())[1]) == _lib.SCAN_CHUNKS_FROM
+
+
+@pytest.mark.gpu
+def test_short_scans_take_no_scratch():
+  """In Python's form of the call, which strided states and the like take, as in the native one."""
+  import recurrentgemma_b200 as rg
+  from recurrentgemma_b200 import _lib
+  from tests.test_state_space import scan_case
+  for t in (1, 40):
+    case = scan_case(t, 2, t, 64, 16, torch.bfloat16)
+    want = rg.selective_scan(**case)
+    wide = torch.empty((2, 64, 32), device="cuda")
+    wide[..., :16] = case["state"]
+    case["state"] = wide[..., :16]
+    rg.selective_scan(**case)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = rg.selective_scan(**case)
+    assert torch.cuda.max_memory_allocated() - held < _lib.load().rgk_selective_scan_workspace_bytes()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
