@@ -557,6 +557,10 @@ RGK_API int rgk_workspace_status(void* workspace, void* stream);
  * aligned; its contents are overwritten. */
 RGK_API int rgk_selftest_wait_expiry(void* workspace, size_t workspace_bytes, void* stream);
 
+/* The same for rgk_selective_scan: a small call in chunks of time whose first chunk is never run.  `status`, a word on the
+ * device (or NULL), must come to hold RGK_ETIMEOUT.  workspace: at least 1 MiB, 256-byte aligned; overwritten. */
+RGK_API int rgk_selftest_scan_wait_expiry(void* workspace, size_t workspace_bytes, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -147,6 +147,7 @@ SIGNATURES = {
     "rgk_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
     "rgk_workspace_status": (_int, [_vp, _vp]),
     "rgk_selftest_wait_expiry": (_int, [_vp, _sz, _vp]),
+    "rgk_selftest_scan_wait_expiry": (_int, [_vp, _sz, _vp, _vp]),
 }
 
 _lib = None

@@ -764,6 +764,36 @@ int rgk_selective_scan(const rgk_scan_inputs* in, const void* segment_pos, int p
   return RGK_OK;
 }
 
+int rgk_selftest_scan_wait_expiry(void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  // A selective scan over 1 sequence x 512 steps x 64 channels x 16 states, cut into four chunks of time whose first
+  // is never run: the second waits for states nobody leaves, gives up after 200 polls (tens of microseconds),
+  // raises the status word and goes on with the states that are there (zeros).
+  const int64_t T = rgk::kScanChunksFrom, E = 64, N = 16;
+  const size_t act = up256(static_cast<size_t>(T * E) * 2), states = up256(static_cast<size_t>(E * N) * 4);
+  const size_t scratch = up256(rgk::selective_workspace_bytes()), need = scratch + 2 * act + 2 * states;
+  RGK_REQUIRE(workspace != nullptr && workspace_bytes >= need, RGK_EWORKSPACE,
+              "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  RGK_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 && aligned_to(status, 4), RGK_EALIGN,
+              "workspace must be 256-byte aligned, status 4-byte");
+  RGK_CHECK_DEVICE();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  char* x = static_cast<char*>(workspace) + scratch;
+  RGK_CUDA(cudaMemsetAsync(x, 0, need - scratch, s), "cudaMemsetAsync");
+  rgk::SelectiveArgs p = {};
+  p.B = 1; p.T = T; p.E = E; p.groups = 1; p.N = static_cast<int>(N);
+  p.x = p.dt = p.b = p.c = x;
+  p.x_token = p.dt_token = p.b_token = p.c_token = E;
+  p.y = x + act;
+  p.a = reinterpret_cast<float*>(x + 2 * act);
+  p.state_out = reinterpret_cast<float*>(x + 2 * act + states);
+  p.ticket = static_cast<unsigned*>(workspace);
+  p.status = status;
+  p.skip_first = 1;
+  p.wait_limit = 200;
+  RGK_CUDA(rgk::launch_selective_scan(p, RGK_BF16, s), "selective scan launch");
+  return RGK_OK;
+}
+
 static_assert(rgk::kScanChunksFrom == RGK_SCAN_CHUNKS_FROM, "as the callers have it");
 size_t rgk_selective_scan_workspace_bytes(void) { return rgk::selective_workspace_bytes(); }
 

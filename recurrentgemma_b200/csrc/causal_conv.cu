@@ -120,7 +120,10 @@ causal_conv_kernel(const ConvArgs p) {
     }
     T* out = static_cast<T*>(p.state_out) + b * kHalo * p.E + e;
 #pragma unroll
-    for (int j = 0; j < kHalo; ++j) *reinterpret_cast<Raw*>(out + (int64_t)j * p.E) = last[j];
+    for (int j = 0; j < kHalo; ++j) {
+      if (RGK_IN_RANGE(out - static_cast<T*>(p.state_out) + j * p.E, p.B * kHalo * p.E - (kPer - 1), nullptr))
+        *reinterpret_cast<Raw*>(out + (int64_t)j * p.E) = last[j];
+    }
   }
 
   T* y = static_cast<T*>(p.y) + (b * p.T + t0) * p.E + e;
@@ -158,7 +161,8 @@ causal_conv_kernel(const ConvArgs p) {
       }
     }
     if (p.silu) silu<T, kPer>(acc);
-    *reinterpret_cast<Raw*>(y + (int64_t)r * p.E) = narrow<T, kPer>(acc);
+    if (RGK_IN_RANGE(y - static_cast<T*>(p.y) + r * p.E, p.B * p.T * p.E - (kPer - 1), nullptr))
+      *reinterpret_cast<Raw*>(y + (int64_t)r * p.E) = narrow<T, kPer>(acc);
   }
 }
 

@@ -357,6 +357,8 @@ struct SelectiveArgs {
   int blocks_per_group;
   int64_t blocks, chunk, chunks;         // of channels; of time: length and number
   int* done;                             // chunks that a block has done
+  int skip_first;                        // the wait-expiry self-test: cut into chunks, the first never run, and a
+  unsigned wait_limit;                   // short limit of polls; else 0
 };
 constexpr int kScanChunksFrom = 512;     // time steps: shorter calls make no use of the scratch
 size_t selective_workspace_bytes();

@@ -152,10 +152,10 @@ template <typename T, int S_, int C_, int L_, int kTile_> struct Shape {
 // Waits until chunk - 1 of a block of channels has left its states.  The CTA that has drawn it is running (all items are
 // drawn in this order, the first one of a CTA too, by CTAs that have started), and none waits for a later one: however
 // few of the CTAs find a place on the device, the item that was drawn first among the unfinished ones goes on.
-__device__ __forceinline__ void wait_for(const int* done, int chunk, int* status) {
+__device__ __forceinline__ void wait_for(const int* done, int chunk, unsigned limit, int* status) {
   if (threadIdx.x == 0) {
     int seen = 0;
-    for (unsigned n = 0; n < kWaitLimit; ++n) {
+    for (unsigned n = 0; n < limit; ++n) {
       asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(done) : "memory");
       if (seen >= chunk) break;
       __nanosleep(200);
@@ -397,6 +397,7 @@ selective_scan_kernel(const SelectiveArgs p) {
             }
           }
           T* to = y + (t0 + t) * p.E + 4 * q;
+          if (!RGK_IN_RANGE(to - static_cast<T*>(p.y), p.B * p.T * p.E - (min(there - 4 * q, 4) - 1), p.status)) continue;
           if (kAligned || (p.store4 && 4 * q + 4 <= there)) {
             if constexpr (sizeof(T) == 2)
               *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3]));
@@ -441,7 +442,7 @@ selective_scan_kernel(const SelectiveArgs p) {
       const int l = tid & (L - 1), owner = tid / L;
       auto channel_of = [&](int c) { const int at = owner + c * Sh::kOwners; return at % kQuads * 4 + at / kQuads; };
       auto state_of = [&](int s) { return s / kRun * kRun * L + l * kRun + s % kRun; };
-      if (chunk > 0) wait_for(p.done + block, (int)chunk, p.status);
+      if (chunk > 0) wait_for(p.done + block, (int)chunk, p.wait_limit, p.status);
       const float* from = chunk > 0 ? p.state_out : p.state_in;
       Pair h[C][S / 2], a2[C][S / 2];
 #pragma unroll
@@ -454,7 +455,8 @@ selective_scan_kernel(const SelectiveArgs p) {
             const int n = state_of(2 * s + i), ch = channel_of(c);
             const bool in = ch < there && n < p.N;
             va[i] = in ? p.a[(first + ch) * p.N + n] * kLog2e : 0.0f;
-            vh[i] = in && from != nullptr ? __ldcg(from + (b * p.E + first + ch) * p.N + n) : 0.0f;
+            vh[i] = in && from != nullptr && RGK_IN_RANGE((b * p.E + first + ch) * p.N + n, p.B * p.E * p.N, p.status)
+                        ? __ldcg(from + (b * p.E + first + ch) * p.N + n) : 0.0f;
           }
           a2[c][s] = pair(va[0], va[1]);
           h[c][s] = pair(vh[0], vh[1]);
@@ -528,7 +530,8 @@ selective_scan_kernel(const SelectiveArgs p) {
           for (int s = 0; s < S; ++s) {
             const int n = state_of(s);
             const float2 v = split(h[c][s / 2]);
-            if (n < p.N) p.state_out[(b * p.E + first + ch) * p.N + n] = s % 2 == 0 ? v.x : v.y;
+            if (n < p.N && RGK_IN_RANGE((b * p.E + first + ch) * p.N + n, p.B * p.E * p.N, p.status))
+              p.state_out[(b * p.E + first + ch) * p.N + n] = s % 2 == 0 ? v.x : v.y;
           }
         }
       }
@@ -536,7 +539,7 @@ selective_scan_kernel(const SelectiveArgs p) {
     if (p.chunks == 1) return;
     __syncthreads();
     if (threadIdx.x == 0) {
-      if (chunk + 1 < p.chunks) {
+      if (chunk + 1 < p.chunks && RGK_IN_RANGE(block, kMostBlocks, p.status)) {
         __threadfence();
         asm volatile("st.release.gpu.global.s32 [%0], %1;" :: "l"(p.done + block), "r"((int)chunk + 1) : "memory");
       }
@@ -559,19 +562,21 @@ cudaError_t launch_kernel(SelectiveArgs p, cudaStream_t s) {
   p.chunks = 1;
   if (p.blocks >= ((int64_t)1 << 31)) return cudaErrorInvalidValue;
   int64_t grid = p.blocks;
+  if (p.wait_limit == 0) p.wait_limit = kWaitLimit;
   // Chunks of time drawn by a ticket.
   if (p.ticket != nullptr && p.state_out != nullptr && p.T >= kScanChunksFrom) {
     int per_sm = 0;
     if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, selective_scan_kernel<T, Sh, kAligned>, 2 * kTeam,
                                                            Sh::kBytes)) != cudaSuccess) return e;
     const int64_t most = min((int64_t)per_sm, p.blocks / sms);
-    if (most > 0 && most * sms < p.blocks && p.blocks <= kMostBlocks) {
-      grid = most * sms;
+    if ((p.skip_first || (most > 0 && most * sms < p.blocks)) && p.blocks <= kMostBlocks) {
+      grid = p.skip_first ? p.blocks : most * sms;
       // (24 of them: the last round is short of 4 % at most; no longer than a wait for one is given)
       p.chunk = min((int64_t)4096, max((int64_t)128, (p.T / 24 + Sh::kTile - 1) / Sh::kTile * Sh::kTile));
       p.chunks = (p.T + p.chunk - 1) / p.chunk;
       p.done = reinterpret_cast<int*>(p.ticket) + 1;
       if ((e = cudaMemsetAsync(p.ticket, 0, (1 + p.blocks) * sizeof(int), s)) != cudaSuccess) return e;
+      if (p.skip_first && (e = cudaMemsetAsync(p.ticket, (int)p.blocks, 1, s)) != cudaSuccess) return e;  // (below 256)
     }
   }
   selective_scan_kernel<T, Sh, kAligned><<<(unsigned)grid, 2 * kTeam, Sh::kBytes, s>>>(p);

@@ -136,3 +136,57 @@ def test_short_scans_take_no_scratch():
     got = rg.selective_scan(**case)
     assert torch.cuda.max_memory_allocated() - held < _lib.load().rgk_selective_scan_workspace_bytes()
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_a_wait_for_a_chunk_expires_and_is_reported():
+  """A call in chunks whose first chunk is never run: the wait for it gives up after 200 polls, the kernel returns, and
+  check_status reports it once; the next call is right."""
+  import recurrentgemma_b200 as rg
+  from recurrentgemma_b200 import _lib
+  from tests.test_state_space import scan_case
+  dev = torch.device("cuda", torch.cuda.current_device())
+  lib = _lib.load()
+  case = scan_case(3, 8, 520, 5120, 16, torch.bfloat16)
+  want = rg.selective_scan(**case)
+  rg.check_status(dev)
+  scratch = torch.empty(1 << 20, dtype=torch.uint8, device=dev)
+  _lib.check(lib.rgk_selftest_scan_wait_expiry(scratch.data_ptr(), scratch.numel(), _lib.status_ptr(dev),
+                                               _lib.stream_ptr(dev)))
+  torch.cuda.synchronize()                          # the kernel has returned by itself
+  with pytest.raises(_lib.RgkError) as err:
+    rg.check_status(dev)
+  assert err.value.code == _lib.RGK_ETIMEOUT
+  rg.check_status(dev)                              # reported once
+  got = rg.selective_scan(**case)
+  rg.check_status(dev)
+  assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_range_checked_build_runs_scans_clean():
+  """librgk_checks.so checks the indices of states, outputs and chunk counters: a bad one would skip its access and show
+  in the status word and the results of the tests that are run on it here."""
+  import subprocess
+  import sys
+  root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+  lib_path = os.path.join(root, "recurrentgemma_b200", "librgk_checks.so")
+  if not os.path.exists(lib_path):
+    pytest.skip("librgk_checks.so not built (python -m recurrentgemma_b200.build --checks)")
+  env = dict(os.environ, RGK_LIBRARY=lib_path)
+  cmd = [sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", os.path.join(root, "tests", "test_scan_chunks.py"),
+         os.path.join(root, "tests", "test_state_space.py"), "-k", "in_chunks or test_selective_scan or test_causal_conv",
+         "-p", "no:cacheprovider"]
+  r = subprocess.run(cmd, env=env, cwd=root, capture_output=True, text=True, timeout=600)
+  assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
+  assert " passed" in r.stdout
+
+
+def test_refusals_of_the_self_test():
+  from recurrentgemma_b200 import _lib, build
+  build.build_library()
+  lib = _lib.load()
+  assert lib.rgk_selftest_scan_wait_expiry(None, 1 << 20, None, None) == _lib.RGK_EWORKSPACE
+  assert lib.rgk_selftest_scan_wait_expiry(256, 1 << 18, None, None) == _lib.RGK_EWORKSPACE
+  assert lib.rgk_selftest_scan_wait_expiry(128, 1 << 20, None, None) == _lib.RGK_EALIGN
+  assert lib.rgk_selftest_scan_wait_expiry(256, 1 << 20, 18, None) == _lib.RGK_EALIGN
