@@ -869,36 +869,41 @@ cudaError_t launch_step_states(const SelectiveArgs& p, int sms, cudaStream_t s) 
 }
 
 // There is a choice of shapes: few states a thread keep a step short where channels are few, many states and two channels
-// share what is read from shared memory where they are many.  What a shape takes, relative: `alone` is its time where every CTA
-// has an SM (us for 1024 steps), the factor what blocks behind the first round of SMs add; a second CTA on an SM costs
-// half as much as the first.
-struct Choice { double alone; int channels; };                   // channels of a CTA
+// share what is read from shared memory where they are many.  What a shape takes for 1024 steps, us: `alone` where every
+// CTA has an SM, and for each round of SMs `some` up to two of them, `many` beyond (where time is cut into chunks).
+struct Choice { double alone, some, many; int channels; };       // channels of a CTA
 template <int kCount>
 int quickest(const Choice (&of)[kCount], const SelectiveArgs& p, int sms) {
   int best = 0;
   double least = 0.0;
-  for (int i = 0; i < kCount; ++i) {
+  for (int i = kCount - 1; i >= 0; --i) {
     const int64_t blocks = (p.per_group + of[i].channels - 1) / of[i].channels * p.groups * p.B;
     const double rounds = (double)blocks / sms;
-    const double time = of[i].alone * (rounds <= 1.0 ? 1.0 : rounds < 2.0 ? rounds + 0.45 : rounds);
-    if (i == 0 || time < least) { best = i; least = time; }
+    const double time = rounds <= 1.0 ? of[i].alone : rounds * (rounds < 2.0 ? of[i].some : of[i].many);
+    // (more channels a CTA fetch b and c less often, which counts where those are not aligned: a tie goes to them)
+    if (i == kCount - 1 || time < 0.96 * least) { best = i; least = time; }
   }
   return best;
 }
 
-// Measured in bfloat16, 1024 steps of 2560 / 10240 / 20480 / 40960 channels (16 states: 2048 steps of 4096 / 10240 / 20480),
-// in the order of the shapes:   8 states 57 / 85 / 113 / 214, 96 / 95 / 133 / 184;   16 states 183 / 292 / 569, 89 / 193 /
-// 372, 134 / 202 / 293, 242 / 240 / 348;   32 states 74 / 194 / 378 / 743, 69 / 142 / 271 / 529, 112 / 155 / 238 / 444;
-// 64 states 120 / 443 / 875 / 1734, 104 / 285 / 554 / 1091, 114 / 236 / 440 / 870;   128 states 168 / 627 / 1237,
-// 191 / 497 / 989.
+// Measured on one B200 with 640 to 40960 channels, in the order of the shapes; a shape's three numbers come from 1024,
+// 1280 to 4096, and 5120 and more.  For instance 2560 / 10240 / 40960 channels, 16 states in float32: 65 / 171 / 643, 54 /
+// 123 / 436, 91 / 130 / 388, 165 / 167 / 439; in bfloat16: 58 / 148 / 553, 46 / 99 / 364, 69 / 103 / 282, 124 / 124 / 277.  64
+// states in float32: 132 / 486 / 1900, 124 / 360 / 1382, 169 / 334 / 1240; in bfloat16: 122 / 450 / 1759, 103 / 283 / 1079,
+// 114 / 237 / 873.
 template <typename T>
 cudaError_t launch_states(const SelectiveArgs& p, int sms, cudaStream_t s) {
+  constexpr bool kF32 = sizeof(T) == 4;
   if (p.N <= 4) return launch<T, 4, 1, 1, 16>(p, s);
   if (p.N <= 8) {
-    return quickest({{57, 64}, {95, 128}}, p, sms) == 0 ? launch<T, 4, 1, 2, 16>(p, s) : launch<T, 4, 2, 2, 16>(p, s);
+    static constexpr Choice f32[] = {{67, 96, 63, 64}, {120, 153, 148, 128}};
+    static constexpr Choice bf16[] = {{57, 79, 51, 64}, {96, 124, 87, 128}};
+    return quickest(kF32 ? f32 : bf16, p, sms) == 0 ? launch<T, 4, 1, 2, 16>(p, s) : launch<T, 4, 2, 2, 16>(p, s);
   }
   if (p.N <= 16) {
-    switch (quickest({{35, 16}, {44.5, 32}, {67, 64}, {121, 128}}, p, sms)) {
+    static constexpr Choice f32[] = {{42, 59, 40, 16}, {54, 77, 55, 32}, {91, 120, 95, 64}, {165, 210, 203, 128}};
+    static constexpr Choice bf16[] = {{35, 53, 35, 16}, {45, 68, 45, 32}, {69, 95, 67, 64}, {124, 168, 128, 128}};
+    switch (quickest(kF32 ? f32 : bf16, p, sms)) {
       case 0: return launch<T, 2, 1, 8, 32>(p, s);
       case 1: return launch<T, 4, 1, 4, 32>(p, s);
       case 2: return launch<T, 8, 1, 2, 16>(p, s);
@@ -906,21 +911,27 @@ cudaError_t launch_states(const SelectiveArgs& p, int sms, cudaStream_t s) {
     }
   }
   if (p.N <= 32) {
-    switch (quickest({{48, 16}, {66, 32}, {112, 64}}, p, sms)) {
+    static constexpr Choice f32[] = {{56, 76, 54, 16}, {85, 111, 86, 32}, {171, 212, 155, 64}};
+    static constexpr Choice bf16[] = {{47, 66, 45, 16}, {68, 92, 65, 32}, {118, 152, 108, 64}};
+    switch (quickest(kF32 ? f32 : bf16, p, sms)) {
       case 0: return launch<T, 4, 1, 8, 32>(p, s);
       case 1: return launch<T, 8, 1, 4, 16>(p, s);
       default: return launch<T, 8, 2, 4, 16>(p, s);
     }
   }
   if (p.N <= 64) {
-    switch (quickest({{65, 8}, {75, 16}, {112, 32}}, p, sms)) {
+    static constexpr Choice f32[] = {{69, 88, 59, 8}, {89, 112, 87, 16}, {169, 203, 150, 32}};
+    static constexpr Choice bf16[] = {{66, 84, 54, 8}, {71, 94, 67, 16}, {114, 143, 106, 32}};
+    switch (quickest(kF32 ? f32 : bf16, p, sms)) {
       case 0: return launch<T, 4, 1, 16, 16>(p, s);
       case 1: return launch<T, 8, 1, 8, 16>(p, s);
       default: return launch<T, 8, 2, 8, 16>(p, s);
     }
   }
   if (p.N <= 128) {
-    return quickest({{86, 8}, {149, 16}}, p, sms) == 0 ? launch<T, 8, 1, 16, 16>(p, s) : launch<T, 8, 2, 16, 8>(p, s);
+    static constexpr Choice f32[] = {{105, 125, 95, 8}, {216, 243, 167, 16}};
+    static constexpr Choice bf16[] = {{83, 104, 74, 8}, {148, 168, 117, 16}};
+    return quickest(kF32 ? f32 : bf16, p, sms) == 0 ? launch<T, 8, 1, 16, 16>(p, s) : launch<T, 8, 2, 16, 8>(p, s);
   }
   return launch<T, 8, 1, 32, 8>(p, s);
 }

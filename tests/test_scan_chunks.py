@@ -190,3 +190,18 @@ def test_refusals_of_the_self_test():
   assert lib.rgk_selftest_scan_wait_expiry(256, 1 << 18, None, None) == _lib.RGK_EWORKSPACE
   assert lib.rgk_selftest_scan_wait_expiry(128, 1 << 20, None, None) == _lib.RGK_EALIGN
   assert lib.rgk_selftest_scan_wait_expiry(256, 1 << 20, 18, None) == _lib.RGK_EALIGN
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,t,e,n,options", [
+    (3, 70, 5120, 8, {}), (3, 70, 5120, 16, dict(part=True)), (1, 70, 2560, 64, {}), (1, 70, 2560, 128, {}),
+    (2, 70, 1280, 32, {}), (1, 70, 1024, 128, dict(part=True))])
+def test_shapes_between_one_round_of_sms_and_two(b, t, e, n, options, dtype):
+  import recurrentgemma_b200 as rg
+  from tests.test_state_space import scan_case, scan_definition, within
+  case = scan_case(n, b, t, e, n, dtype, 1, 20, **options)
+  y, state = rg.selective_scan(**case)
+  want, held, bound, bound_state = scan_definition(**case)
+  within(y, want, bound, dtype)
+  within(state, held, bound_state, torch.float32)
