@@ -499,9 +499,9 @@ RGK_API int rgk_geglu_bias(const void* up, const void* bias, int64_t M, int64_t 
  *   that a wait which gives up raises to RGK_ETIMEOUT (a workspace's first int), or NULL.
  * rgk_sample: out [M] int32, one token for each row of logits [M,V] (rows row_stride apart; V up to 2^20).
  *   Tokens are ordered by logit, the largest first, equal ones by index.  Kept are the first top_k of them (all for
- *   top_k <= 0), of those, with weights exp((logit - largest) / temperature) rounded to multiples of 2^-44
- *   (2^-43 above 2^18 tokens, 2^-42 above 2^19), the shortest prefix with at least top_p of their weight (one at least;
- *   all for top_p >= 1), of those the ones with at least min_p of the largest weight.  The token is the first, by index, up to which the kept weights sum
+ *   top_k <= 0), of those, with weights exp((logit - largest) / temperature), the shortest prefix with at least top_p of
+ *   their weight (one at least; all for top_p >= 1), of those the ones with at least min_p of the largest weight.
+ *   Weights are held as multiples of 2^-44 (2^-43 above 2^18 tokens, 2^-42 above 2^19), each within one of those.  The token is the first, by index, up to which the kept weights sum
  *   to more than uniforms[m] (in [0, 1)) times all of them.  A temperature of 0 (or less) takes the
  *   first maximum.  NaN counts as -inf; neither is drawn; a row of nothing else gives 0.
  *   Every setting is an array of M on the device, or NULL: the value beside it for all rows.

@@ -1,6 +1,6 @@
 // One token per row of logits: temperature, top-k, top-p and min-p, drawn by a given uniform number.
 //
-// Weights are integers: W(l) = 2^F exp((l - max) / T), rounded, with F = 44 or as many bits as keep the sum of a row
+// Weights are integers: W(l) = 2^F exp((l - max) / T), to within one, with F = 44 or as many bits as keep the sum of a row
 // below 2^62.  Sums of integers do not depend on their order, so that a row gives the same token whatever the launch,
 // and 44 bits make the borders between tokens finer than a float32 sum over 256000 of them could (whose rounding would
 // move a border by a few percent of such a token's width).  Order: logit descending, ties by lowest index.
@@ -56,7 +56,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 // 2^F exp((l - max) / T): 2^t with t = n + j / 64 + f, |f| <= 1/128, as 2^n, a table of 2^(j / 64) and the Taylor
-// polynomial of 2^f to degree 4 (4e-14 of the value).  Of tokens within 44 temperatures of the maximum: the callers
+// polynomial of 2^f to degree 4 (4e-14 of the value, 0.7 of the last bit of the largest weight).  Of tokens within 44 temperatures of the maximum: the callers
 // drop what it says of others.  No branches: the tokens of a pack are evaluated side by side.
 struct Weights {
   double scale;                                                   // log2(e) / T

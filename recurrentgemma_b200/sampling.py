@@ -35,9 +35,9 @@ def sample(
   """One token (int32) for every row of logits [..., V], drawn by the row's uniform number in [0, 1).
 
   Tokens are ordered by logit, largest first, equal ones by index.  Kept are the first `top_k` (0: all); of
-  those, with weights exp((logit - largest) / temperature) rounded to multiples of 2**-44 (2**-43 above
-  2**18 tokens, 2**-42 above 2**19), the shortest prefix with at least `top_p` of their weight (1: all); of those the ones with at
-  least `min_p` of the largest weight.  The token is the first by index up to which the kept weights sum to
+  those, with weights exp((logit - largest) / temperature), the shortest prefix with at least `top_p` of their
+  weight (1: all); of those the ones with at least `min_p` of the largest weight.  Weights are held as multiples of
+  2**-44 (2**-43 above 2**18 tokens, 2**-42 above 2**19), each within one of those.  The token is the first by index up to which the kept weights sum to
   more than `uniforms` times all of them.  Temperature 0 takes the first maximum.
   NaN counts as -inf and neither is ever drawn; a row of nothing else gives 0.
 

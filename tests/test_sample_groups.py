@@ -61,3 +61,51 @@ def test_settings_of_rows_below_their_range():
   assert torch.equal(rg.sample(logits, u, min_p=row(-2.0)), every)
   assert torch.equal(rg.sample(logits, u, top_k=torch.full((6,), -9, dtype=torch.int32, device="cuda")), every)
   assert torch.equal(rg.sample(logits, u, min_p=row(7.0)), rg.sample(logits, u, min_p=1.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [31, 5000, 50257])
+def test_temperatures_of_any_size(v, dtype):
+  import recurrentgemma_b200 as rg
+  logits, u, _ = rows(v, 5, v, dtype)
+  logits[1, ::2] = torch.finfo(dtype).min
+  logits[2, 3], logits[2, 9] = torch.finfo(dtype).max, torch.finfo(dtype).min
+  logits[3, ::3] = -math.inf
+  logits[4] = logits[4].abs() * -1e-3
+  logits[4, 11] = 0.0
+  for t in (1e-45, 1e-38, 1e-30, 1e-3, 300.0, 1e30, 3e38, math.inf):
+    for settings in ({}, dict(top_k=20), dict(top_p=0.7), dict(top_k=300, top_p=0.9, min_p=0.5)):
+      assert torch.equal(rg.sample(logits, u, temperature=t, **settings),
+                         definition(logits, u, temperature=t, **settings)), (t, settings)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [1000, 50257, 256000, 2 ** 18 + 5, 2 ** 20])
+def test_rounding_of_the_weights(v):
+  """Against weights in 64 bits, not rounded to the kernel's: each of the kernel's is within one multiple of 2^-44 (-43, -42)
+  of them, so that a sum is within v of those.  Where no border is nearer than that the token is the same.  (v borders twice
+  2 v units wide in a sum of some hundred: a row in two hundred at 2^20 tokens, fewer below; one of sixteen may be left out.)"""
+  import recurrentgemma_b200 as rg
+  unit = 2.0 ** -(44 if v <= 2 ** 18 else 43 if v <= 2 ** 19 else 42)
+  logits, u, _ = rows(v, 16, v, torch.float32)
+  order = torch.sort(logits, dim=-1, descending=True, stable=True).indices
+  sorted_logits = torch.gather(logits, 1, order).double()
+  far = 2.0 * v * unit                                # (a border's sum, and the target, which is a share of another sum)
+  for t, p in ((1.0, 1.0), (2.5, 1.0), (1.0, 0.9), (0.7, 0.5)):
+    share = float(torch.tensor(p, dtype=torch.float32))
+    w = torch.exp((sorted_logits - sorted_logits[:, :1]) / float(torch.tensor(t, dtype=torch.float32)))
+    upto = torch.cumsum(w, -1)
+    sure = torch.ones(16, dtype=torch.bool, device="cuda")
+    if p < 1.0:
+      target = share * upto[:, -1:]
+      sure &= (upto - target).abs().min(-1).values > far
+      w = torch.where(upto - w < target, w, 0.0)
+    w = torch.zeros_like(w).scatter_(1, order, w)
+    upto = torch.cumsum(w, -1)
+    target = u.double()[:, None] * upto[:, -1:]
+    sure &= (upto - target).abs().min(-1).values > far
+    want = (upto <= target).sum(-1).int()
+    got = rg.sample(logits, u, temperature=t, top_p=p)
+    assert torch.equal(got[sure], want[sure])
+    assert sure.sum() >= 15
