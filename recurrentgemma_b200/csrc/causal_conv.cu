@@ -7,7 +7,7 @@
 // Bound: HBM, every element is read and written once.  A thread owns one pack of channels (8 bytes, or one
 // channel where the rows are not aligned to that) and kRows consecutive rows, whose loads are all asked for before
 // the first is used; the W-1 rows in front of them come from L2, where the neighbour has just put them.  8 x 4096 x
-// 5120 in bfloat16: 124 us, 83 % of the measured copy rate (with packs of 16 bytes, 160 registers a thread, 168).
+// 5120 in bfloat16: 119 us, 86 % of the measured copy rate (with packs of 16 bytes, 160 registers a thread, 168).
 #include "packed.cuh"
 #include "rgk_common.cuh"
 #include "rgk_internal.h"

@@ -6,7 +6,7 @@
 // Bound: the special functions.  An (element, state) takes one exponential and four multiply-adds' worth of
 // float32 work, and an SM has 16 special-function results a clock but 128 multiply-adds: for 16 states (and
 // three more for softplus and silu) 168 M elements take 0.71 ms where their bytes take 0.21.  8 x 4096 x 5120 in
-// bfloat16: 988 us, 72 % of that rate.
+// bfloat16: 995 us, 71 % of that rate.  (In float32 the decays take a polynomial as well: exact_decays.)
 //
 // The recurrence runs in time order in registers: L neighbouring lanes share a channel, each with S of its
 // states, and time is not split - the lanes are, which leaves no work to do twice.  A CTA is two teams of 128 threads.
