@@ -666,7 +666,8 @@ sample_kernel(const SampleArgs p, int parts) {
     if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
   };
   // (In a row that begins inside of a pack a group may be without a token, or not be asked: a bound it is all the same.)
-  const bool fine = top_k_of(p, m) > p.coarse.most_k;
+  const int k = top_k_of(p, m);
+  const bool fine = k > p.coarse.most_k && k <= kMostK;
   const int group = fine ? p.fine.lanes : p.coarse.lanes;
   float of_group = best;
 #pragma unroll

@@ -60,13 +60,22 @@ __device__ __forceinline__ float2 softplus_steps(float v0, float v1) {
 // In float32, and up to 4 states (of a channel, rounded up), the decays are exp2_exact: slow states keep their terms for a
 // thousand steps, and that the hardware's exponential is a little small shows in them.  2048 steps of 1 / 8 / 16 states in
 // float32: 1.2e-6 / 7.8e-7 / 6.0e-7 off 64 bits with it, 2.1e-7 / 1.7e-7 / 1.5e-7 so, for 2 / 5 / 24 % more time (a step of
-// 256 sequences 45 -> 48 us).  bfloat16 calls of more states keep the hardware's: 16 of them 6.1e-7 off, where 1.4e-7
-// would take 30 % longer.  One rule for sequences and single steps, so that they come to the same states.
+// 256 sequences 45 -> 48 us).  bfloat16 calls of more states keep the hardware's (30 % more time otherwise), of an argument
+// that is 2e-8 larger, which costs nothing and takes most of the bias away: its mean error, in 1e-9, for |x| from 1e-5 / 1e-4 /
+// 1e-3 / 1e-2 / 0.05 / 0.1 / 0.2 up to the next is -8 / -6 / -12 / -26 / -14 / -18 / -20, and +6 / +8 / +2 / -12 / +1 / -6 /
+// -2 so (rms 30 to 47, and 30 to 35); a step of 0 still is a factor of 1.  One rule for sequences and single steps, so that they
+// come to the same states.
+constexpr float kDecayBias = 2.0e-8f;
 template <typename T> constexpr bool exact_decays(int states) { return sizeof(T) == 4 || states <= 4; }
 // 2^(step a) for two states
+template <bool kExact> __device__ __forceinline__ Pair decays(Pair step, Pair a) {
+  if constexpr (kExact) return exp2_exact(mul2(step, a));
+  else return exp2_pair(fma2(step, a, pair(kDecayBias, kDecayBias)));
+}
+// (not packed without the polynomial: one register less for the constant)
 template <bool kExact> __device__ __forceinline__ float2 decays(float step, float a0, float a1) {
-  const Pair arg = mul2(pair(step, step), pair(a0, a1));
-  return split(kExact ? exp2_exact(arg) : exp2_pair(arg));
+  if constexpr (kExact) return split(decays<true>(pair(step, step), pair(a0, a1)));
+  else return make_float2(exp2_fast(fmaf(step, a0, kDecayBias)), exp2_fast(fmaf(step, a1, kDecayBias)));
 }
 
 // four consecutive elements, at an address aligned to four of them
@@ -500,10 +509,9 @@ selective_scan_kernel(const SelectiveArgs p) {
                 Pair both = 0;
 #pragma unroll
                 for (int s = 0; s < S / 2; ++s) {
-                  const Pair arg = mul2(step2, a2[c][s]);
                   Pair before = h[c][s];
                   if (decltype(with_starts)::value && ((starts >> t) & 1u)) before = 0;
-                  h[c][s] = fma2(kExact ? exp2_exact(arg) : exp2_pair(arg), before, mul2(put2, vb[s]));
+                  h[c][s] = fma2(decays<kExact>(step2, a2[c][s]), before, mul2(put2, vb[s]));
                   both = s == 0 ? mul2(h[c][s], vc[s]) : fma2(h[c][s], vc[s], both);
                 }
                 const float2 halves = split(both);
@@ -729,7 +737,7 @@ selective_step_kernel(const SelectiveArgs p) {
 // The same for many sequences: a thread goes through kDepth and more of them with the same four states of a channel, whose
 // values come by copies that run kDepth sequences ahead into places of its own in shared memory (nobody else reads them:
 // no barriers), the rest of a sequence a step ahead into registers.  256 x 5120 x 16 in bfloat16: 48 us with
-// four sequences a thread, 43 so (64 % of the measured copy rate).
+// four sequences a thread, 44 so (63 % of the measured copy rate).
 // (Addresses run along: products of 64 bits for every row were most of its 237 instructions, which bound it.)
 template <typename T, int L>
 __global__ void __launch_bounds__(256, 4)

@@ -109,8 +109,8 @@ def selective_scan(
   float32 is h in front of the first token (None: zeros); a decode step is a call with one token.  A document
   start (segment_pos == 0) drops the state in front of it.  `inplace` overwrites `state` and returns it.
   Decay factors and steps are float32 evaluations as exact as the formula's in float32; bfloat16 calls with more than
-  4 states take the hardware's exponential for the factors, which is a little small near 1: after 2048 steps their states
-  are 6e-7 off 64 bits (2-norm), where float32 calls are 1.5e-7.
+  4 states take the hardware's exponential for the factors: after 2048 steps their states are 3e-7 off 64 bits
+  (2-norm), where float32 calls are 1.5e-7.
   x, dt, z, b and c may be strided over batch and time.  Where x or a step is infinite, y may be NaN instead of
   infinite; the states are as the formula has them.
   """

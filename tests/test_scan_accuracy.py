@@ -168,3 +168,45 @@ def test_gate_in_float32(b, t):
   got = rg.selective_scan(**case)[0][..., :6]
   want = (case["d"] * case["x"] * (case["z"] / (1.0 + torch.exp(-case["z"]))))[..., :6]
   assert torch.equal(got.isnan(), want.isnan()) and torch.allclose(got.nan_to_num(), want.nan_to_num(), rtol=1e-6, atol=1e-30)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("single", [False, True])
+@pytest.mark.parametrize("lo,hi", [(1e-5, 1e-4), (1e-4, 1e-3), (1e-3, 1e-2), (1e-2, 1e-1)])
+def test_slow_states_of_bfloat16_calls(lo, hi, single):
+  """1000 steps of states with decay rates of lo to hi a step, in bfloat16, where the factors are the hardware's.  Up to 1e-2
+  no further off than the formula in float32.  Beyond, the mean error of a factor (13e-9 at most) counts as often as a term
+  is old, 1 / (2 lo) steps, and its random part with the multiply-add's (0.69 u) by the root of that: 6.5e-7 and 2.9e-7."""
+  import recurrentgemma_b200 as rg
+  t, e, n = 1000, 320, 16
+  g = torch.Generator(device="cuda").manual_seed(3)
+  case = layer(4, 1, t, e, n, torch.bfloat16, False)
+  case["dt"] = (0.5 + torch.rand((1, t, e), generator=g, device="cuda")).bfloat16()
+  case["a"] = -torch.exp(torch.rand((e, n), generator=g, device="cuda") * math.log(hi / lo) + math.log(lo))
+  state = torch.randn((1, e, n), generator=g, device="cuda")
+
+  def formula(dtype):
+    h, (x, dt, a, b) = state.to(dtype), (case[k].to(dtype) for k in ("x", "dt", "a", "b"))
+    for i in range(t):
+      h = torch.exp(dt[:, i, :, None] * a) * h + (dt[:, i] * x[:, i])[:, :, None] * b[:, i]
+    return h
+  want, plain, got = formula(torch.float64), formula(torch.float32), state.clone()
+  for i in range(0, t, 1 if single else t):
+    part = {k: case[k][:, i:i + 1] if single else case[k] for k in ("x", "dt", "b", "c")}
+    rg.selective_scan(**part, a=case["a"], state=got, softplus=False, inplace=True)
+  assert off(got, want) <= (off(plain, want) if hi <= 1e-2 else math.hypot(6.5e-7, 2.9e-7))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [3, 16, 21])
+def test_steps_of_no_time_leave_the_states(n, dtype):
+  """A step of 0, given or as softplus of -infinity, is a factor of exactly 1 and puts nothing in."""
+  import recurrentgemma_b200 as rg
+  for t in (1, 45):
+    case = layer(n, 70, t, 640, n, dtype)
+    state = torch.randn((70, 640, n), generator=torch.Generator(device="cuda").manual_seed(n), device="cuda")
+    for dt, softplus in ((0.0, False), (-math.inf, True)):
+      case["dt"] = torch.full_like(case["dt"], dt)
+      given = {**case, "dt_bias": None} if not softplus else case
+      assert torch.equal(rg.selective_scan(**given, state=state, softplus=softplus)[1], state)
